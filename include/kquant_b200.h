@@ -338,6 +338,58 @@ KQ_API int kq_gather_qmm_seg(const void* x, int x_dtype, long long rows, int K, 
                              const uint32_t* map, const uint32_t* count, long long map_tiles, void* y, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ---- routing to experts in groups, and its gradient (no counterpart in the reference) ----
+ * kq_moe_router_grouped: logits [T, E] of `dtype`, scores s = "sigmoid" or "softmax" of them in float32. Experts are ranked by
+ *   q = s + bias [E] (NULL: by the logits themselves, which rank alike), in 64 bits where that is a sum. The E experts are
+ *   n_groups groups of E / n_groups neighbours; a group counts by the sum of its group_top (1 or 2) largest q, the top_groups
+ *   best groups stay, and of these the top_k largest q are picked, lowest index first among equals. weights float32 [T, top_k]
+ *   = scale * s / (sum of the picked s + 1e-20), or scale * s without norm_topk_prob; indices int32 [T, top_k].
+ *   An expert whose logit (or bias) is -infinity is not available; where fewer than top_k are, the rest of the row is index -1 with
+ *   weight 0, which the expert products skip. A NaN logit is picked first and makes the row's weights NaN (with sigmoid and
+ *   without norm_topk_prob its own alone). E <= 1024, top_k <= 32, E a multiple of n_groups.
+ * kq_moe_router_grouped_backward: dlogits [T, E] of `dtype` from dweights float32 [T, top_k], for the same logits and the indices
+ *   that the call above gave (the bias and the groups only choose: they have no gradient). */
+KQ_API int kq_moe_router_grouped(const void* logits, int dtype, long long T, int E, int top_k, int n_groups, int top_groups,
+                                 int group_top, const char* scoring, const float* bias, int norm_topk_prob, float scale,
+                                 int32_t* indices, float* weights, void* stream);
+KQ_API int kq_moe_router_grouped_backward(const void* logits, int dtype, long long T, int E, int top_k, const char* scoring,
+                                          int norm_topk_prob, float scale, const int32_t* indices, const float* dweights,
+                                          void* dlogits, void* stream);
+
+/* ---- low-rank adapters of many requests beside a shared projection or expert stack (no counterpart in the reference) ----
+ * rows entries e = token * slots + slot, each with a group g = adapter * n_experts + expert: adapter = adapter_ids[token] (int32,
+ * rows / slots of them; NULL: 0), expert = experts[e] (uint32; NULL: 0). An entry whose adapter is outside [0, n_adapters) or whose
+ * expert is outside [0, n_experts) has none: its row of out is y's. f = scale * scaling[adapter] (scaling: float32, or NULL: 1).
+ *  kq_lora_update: out[e] = y[e] + f (x[e] . a[g]^T) . b[g]^T; x rows of K values (x_shared != 0: one row per token, else one per
+ *    entry), a [n_adapters, n_experts, rank, K], b [n_adapters, n_experts, N, rank], y and out rows of N values; out may be y.
+ *    float32 sums, one rounding to out. u: NULL, or float32 [rows, rank] that receives x . a^T (what the gradient needs; zero
+ *    for entries without a group).
+ *  kq_lora_backward, from dy [rows, N] and that u: dx (rows of x, contiguous in K) = f (dy . b[g]) . a[g], summed over a token's slots
+ *    where x_shared; da and db, of the parameters' type and shape, whole (zero for groups without entries). Each may be NULL. What
+ *    flows to y is dy itself.
+ *  dtype: of x, y, out, dy, dx: KQ_F16 or KQ_BF16; param_dtype: of a, b, da, db: the same, or KQ_F32. rank <= 128. Row strides in
+ *    elements, rows dense. Any K, N, rank and alignment; whole groups of 16 bytes are faster.
+ *  plan: the entries in the order of their groups, made by kq_lora_plan in kq_lora_plan_bytes(rows, n_adapters * n_experts)
+ *    bytes of device memory (256-byte aligned) for the same adapter_ids, experts, rows, slots, n_adapters, n_experts. Needed by
+ *    kq_lora_backward unless adapter_ids and experts are both NULL; kq_lora_update takes NULL too, but then looks for the rows of each
+ *    group in every call: meant for up to 128 entries.
+ *  workspace: kq_lora_backward_workspace_bytes(...) bytes, 256-byte aligned, private to the call until it completes.
+ *  The same call gives the same bits. rows < 2^31, n_adapters * n_experts <= 65535. */
+KQ_API size_t kq_lora_plan_bytes(long long rows, int n_groups);
+KQ_API int kq_lora_plan(const int32_t* adapter_ids, const uint32_t* experts, long long rows, int slots, int n_adapters,
+                        int n_experts, void* plan, size_t plan_bytes, void* stream);
+KQ_API int kq_lora_update(const void* x, int dtype, long long rows, int K, long long x_row_stride, int slots, int x_shared,
+                          const void* a, const void* b, int param_dtype, int rank, int N, int n_adapters, int n_experts,
+                          const int32_t* adapter_ids, const uint32_t* experts, const float* scaling, float scale, const void* y,
+                          long long y_row_stride, void* out, long long out_row_stride, float* u, const void* plan,
+                          size_t plan_bytes, void* stream);
+KQ_API size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int rank);
+KQ_API int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long dy_row_stride, const void* x, int K,
+                            long long x_row_stride, int slots, int x_shared, const void* a, const void* b, int param_dtype,
+                            int rank, int n_adapters, int n_experts, const int32_t* adapter_ids, const uint32_t* experts,
+                            const float* scaling, float scale, const float* u, void* dx, void* da, void* db, const void* plan,
+                            size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,8 +9,9 @@ reference's names, argument order and defaults (bindings.cpp:40-43, 94-141,
 ``include/kquant_b200.h``; importing this package without the built library
 raises at the first op call.
 """
+from .lora import lora_update, quantized_matmul_lora
 from .ops import (codec_geometry, codecs, dequantize, expert_tile_map, gather_qmm, gather_qmm_seg, quantize,
                   quantized_matmul, quantized_matmul_qmv_bias)
 
 __all__ = ["codecs", "codec_geometry", "dequantize", "quantized_matmul", "gather_qmm", "quantize", "expert_tile_map",
-           "gather_qmm_seg", "quantized_matmul_qmv_bias"]
+           "gather_qmm_seg", "quantized_matmul_qmv_bias", "lora_update", "quantized_matmul_lora"]

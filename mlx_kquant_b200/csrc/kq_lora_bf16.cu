@@ -1,0 +1,8 @@
+// The tile kernels of bf16 rows and bf16 parameters (kq_lora.cuh).
+#include "kq_lora.cuh"
+
+namespace kq {
+cudaError_t launch_lora_tile_bf16(const LoraArgs& a, bool backward, int mt, int cluster, cudaStream_t st) {
+  return lora::launch_types<lora::bf16, lora::bf16>(a, backward, mt, cluster, st);
+}
+}  // namespace kq

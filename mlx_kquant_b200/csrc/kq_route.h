@@ -1,0 +1,20 @@
+// Internal interface of the grouped router (kq_route.cu) to its C entry points.
+#pragma once
+
+#include <cuda_runtime.h>
+
+namespace kq {
+
+struct RouteArgs {
+  const void* logits;  // [T, E]
+  int dtype, T, E, G, top_groups, group_top, top_k, scoring, norm;  // scoring: 0 softmax, 1 sigmoid
+  const float* bias;   // [E] or nullptr
+  float scale;
+  int* indices;        // [T, top_k]
+  float* weights;      // [T, top_k]
+  const float* dw;     // [T, top_k]  (gradient only)
+  void* dlogits;       // [T, E], or nullptr: the forward pass
+};
+cudaError_t launch_route(const RouteArgs& a, cudaStream_t st);
+
+}  // namespace kq

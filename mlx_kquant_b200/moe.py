@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import gather_qmm
+from .ops import _on_device, _stream_ptr, gather_qmm
 
 
 def route_topk(router_logits: torch.Tensor, top_k: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -818,3 +818,151 @@ def moe_router_topk(logits, top_k, norm_topk_prob, shared_gate=True, per_expert_
     if shared_gate:
         picked = torch.cat([picked, torch.sigmoid(lf[:, E:E + 1])], dim=1)
     return idx.to(torch.int32), picked
+
+
+def _route_grouped_host(logits, top_k, n_groups, top_groups, scoring, bias, group_top, norm_topk_prob, scale):
+    """moe_router_grouped for host tensors, the same computation in torch ops."""
+    T, E = logits.shape
+
+    def scores(x):
+        if scoring == "sigmoid":
+            return torch.sigmoid(x)
+        most = x.amax(dim=1, keepdim=True)
+        e = torch.exp(x - torch.where(most == -torch.inf, 0.0, most))
+        total = e.sum(dim=1, keepdim=True)
+        return e / torch.where(total == 0.0, 1.0, total)
+
+    x = logits.detach().double()
+    rank = x if bias is None else scores(x) + bias.double()
+    by = scores(x) if bias is None and group_top > 1 else rank
+    gone = (x == -torch.inf) | (rank == -torch.inf)
+    rank, by = (torch.where(gone, -torch.inf, torch.where(t != t, torch.inf, t)) for t in (rank, by))
+    if top_groups < n_groups:
+        best = torch.sort(by.view(T, n_groups, -1), dim=2, descending=True).values[:, :, :group_top]
+        total = best[:, :, 0] if best.shape[2] == 1 else best[:, :, 0] + torch.where(best[:, :, 1] == -torch.inf, 0.0, best[:, :, 1])
+        order = torch.sort(total, dim=1, descending=True, stable=True).indices[:, :top_groups]
+        kept = torch.zeros((T, n_groups), dtype=torch.bool).scatter_(1, order, True).repeat_interleave(E // n_groups, dim=1)
+        rank = torch.where(kept, rank, -torch.inf)
+    ranked = torch.sort(rank, dim=1, descending=True, stable=True)
+    idx, some = ranked.indices[:, :top_k], ranked.values[:, :top_k] > -torch.inf
+    picked = torch.where(some, torch.gather(scores(logits.float()), 1, idx), 0.0)
+    if norm_topk_prob:
+        picked = picked / (picked.sum(dim=1, keepdim=True) + 1e-20)
+    return torch.where(some, idx, -1).to(torch.int32), picked * float(scale)
+
+
+class _RouteGrouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, args):
+        idx, w = _route_grouped(logits, *args)
+        ctx.args = args
+        ctx.save_for_backward(logits, idx)
+        ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)
+        return idx, w
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _, dw):
+        if dw is None:
+            return None, None
+        logits, idx = ctx.saved_tensors
+        top_k, _, _, scoring, _, _, norm, scale = ctx.args
+        lc, dw = logits.contiguous(), dw.contiguous()
+        T, E = lc.shape
+        out = torch.empty_like(lc)
+        with torch.cuda.device(lc.device):
+            _lib.check(_lib.lib().kq_moe_router_grouped_backward(
+                lc.data_ptr(), _DT[lc.dtype], T, E, top_k, scoring.encode(), int(norm), scale, idx.data_ptr(), dw.data_ptr(),
+                out.data_ptr(), torch.cuda.current_stream(lc.device).cuda_stream))
+        return out, None
+
+
+def _route_grouped(logits, top_k, n_groups, top_groups, scoring, bias, group_top, norm, scale):
+    lc = logits.contiguous()
+    T, E = lc.shape
+    dev = lc.device
+    idx = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        _lib.check(_lib.lib().kq_moe_router_grouped(
+            lc.data_ptr(), _DT[lc.dtype], T, E, top_k, n_groups, top_groups, group_top, scoring.encode(),
+            bias.data_ptr() if bias is not None else None, int(norm), scale, idx.data_ptr(), w.data_ptr(), _stream_ptr(None, dev)))
+    return idx, w
+
+
+def moe_router_grouped(logits, top_k, n_groups=1, top_groups=1, *, scoring="sigmoid", bias=None, group_top=2,
+                       norm_topk_prob=True, scale=1.0):
+    """Routing to experts in groups, with a bias for balance: score the E columns of logits [T, E] ("sigmoid" or "softmax", in
+    float32), keep the `top_groups` of the `n_groups` groups of neighbouring experts whose `group_top` (1 or 2) largest scores
+    (+ `bias` [E]) have the largest sum, pick of these the `top_k` experts with the largest score (+ bias), lowest index first
+    among equals. The weights are the picked scores without the bias, renormalised to 1 with `norm_topk_prob` (over their sum
+    + 1e-20), times `scale`. What is ranked is compared as in 64 bits.
+
+    An expert with a logit of -inf is not available: where fewer than top_k are, the row ends in index -1 with weight 0 (the expert
+    products skip such entries). A NaN logit comes first and makes the row's weights NaN (with sigmoid and without norm_topk_prob its own alone).
+
+    Returns (indices [T, top_k] int32, weights [T, top_k] float32), the index type and the weights that `moe_glu` and the fused ops
+    take; the weights are differentiable in the logits (CUDA tensors: one kernel each way; host tensors: torch ops).
+    E <= 1024, top_k <= 32."""
+    op = "moe_router_grouped"
+    if scoring not in ("sigmoid", "softmax"):
+        raise ValueError(f"[mlx_kquant.{op}] unknown scoring '{scoring}'.")
+    if logits.dim() != 2 or logits.dtype not in _DT:
+        raise ValueError(f"[mlx_kquant.{op}] logits must be floating [T, E] but got {logits.dtype} {tuple(logits.shape)}.")
+    E = logits.shape[1]
+    if E < 1 or E > 1024 or top_k < 1 or top_k > 32 or top_k > E:
+        raise ValueError(f"[mlx_kquant.{op}] needs 1 <= top_k <= min(E, 32) and E <= 1024.")
+    if n_groups < 1 or E % n_groups != 0 or top_groups < 1 or top_groups > n_groups:
+        raise ValueError(f"[mlx_kquant.{op}] needs E a multiple of n_groups and 1 <= top_groups <= n_groups.")
+    if group_top not in (1, 2):
+        raise ValueError(f"[mlx_kquant.{op}] group_top must be 1 or 2.")
+    if top_groups * (E // n_groups) < top_k:
+        raise ValueError(f"[mlx_kquant.{op}] the kept groups have fewer than top_k experts.")
+    if bias is not None:
+        if bias.shape != (E,):
+            raise ValueError(f"[mlx_kquant.{op}] bias must be of shape ({E},) but has {tuple(bias.shape)}.")
+        bias = bias.detach().to(device=logits.device, dtype=torch.float32).contiguous()
+    args = (top_k, n_groups, top_groups, scoring, bias, group_top, bool(norm_topk_prob), float(scale))
+    if not logits.is_cuda:
+        return _route_grouped_host(logits, *args)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _RouteGrouped.apply(logits, args)
+    return _route_grouped(logits, *args)
+
+
+def gather_lora_update(y, x, a, b, indices, adapter_ids=None, scaling=None, *, out=None, stream=None):
+    """Low-rank adapters of many requests beside an expert stack: slot (t, j), which goes to expert e = indices[t, j], gets
+    ``y[t, j] + scaling[g] * (x @ a[g, e].T) @ b[g, e].T`` with the adapter g = adapter_ids[t] of its token.
+
+    y [T, R, N]: the slots' products (`gather_qmm`, `moe_glu_gather_kq` shapes), float16 or bfloat16; x [T, K], one row per token, or
+    [T, R, K], one per slot; a [G, E, r, K] and b [G, E, N, r] (without the first axis: one adapter for all); indices [T, R];
+    adapter_ids [T], None: adapter 0. A slot whose expert is outside [0, E) or whose adapter is outside [0, G) stays y's. The rest is
+    as in `lora_update`."""
+    from .lora import _Call, _i32, _update
+
+    op = "gather_lora_update"
+    if a.dim() == 3 and b.dim() == 3:
+        a, b = a.unsqueeze(0), b.unsqueeze(0)
+    if a.dim() != 4 or b.dim() != 4:
+        raise ValueError(f"[mlx_kquant.{op}] a must be [adapters, experts, r, K] and b [adapters, experts, N, r] but got shapes "
+                         f"{tuple(a.shape)}, {tuple(b.shape)}.")
+    if indices.dim() != 2 or y.dim() != 3 or y.shape[:2] != indices.shape:
+        raise ValueError(f"[mlx_kquant.{op}] y must be [T, R, N] and indices [T, R] but got {tuple(y.shape)}, {tuple(indices.shape)}.")
+    if x.dim() not in (2, 3) or x.shape[:-1] != indices.shape[:x.dim() - 1]:
+        raise ValueError(f"[mlx_kquant.{op}] x must be [T, K] or [T, R, K] but got {tuple(x.shape)} for indices {tuple(indices.shape)}.")
+    if indices.is_floating_point() or indices.dtype == torch.bool:
+        raise ValueError(f"[mlx_kquant.{op}] indices must be integers but are {indices.dtype}.")
+    call = _Call()
+    call.shared, call.n_experts, call.slots, call.ids = x.dim() == 2, a.shape[1], max(1, indices.shape[1]), None
+    if a.shape[0] * a.shape[1] > 65535:
+        raise ValueError(f"[mlx_kquant.{op}] needs adapters * experts <= 65535.")
+    if adapter_ids is not None:
+        if adapter_ids.shape != indices.shape[:1] or adapter_ids.is_floating_point() or adapter_ids.dtype == torch.bool:
+            raise ValueError(f"[mlx_kquant.{op}] adapter_ids must be integers of shape ({indices.shape[0]},) but got "
+                             f"{adapter_ids.dtype} {tuple(adapter_ids.shape)}.")
+        call.ids = _i32(adapter_ids, x.device)
+    elif a.shape[0] != 1:
+        raise ValueError(f"[mlx_kquant.{op}] {a.shape[0]} adapters need adapter_ids.")
+    call.experts = _i32(indices, x.device)
+    return _update(op, y, x, a, b, call, scaling, out, stream)

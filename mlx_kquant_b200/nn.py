@@ -1,5 +1,6 @@
 """torch modules over GGUF wire bytes, the counterparts of the reference's module layer
-(mlx_kquant/nn.py:50-268): `KQuantEmbedding`, `KQuantLinear`, `KQuantSwitchLinear`.
+(mlx_kquant/nn.py:50-268): `KQuantEmbedding`, `KQuantLinear`, `KQuantSwitchLinear`, and low-rank adapters on the last two:
+`KQuantLoRALinear`, `KQuantLoRASwitchLinear`.
 
 Each keeps `weight` as a uint8 buffer of wire bytes (never a float copy) and a one-byte `scales`
 placeholder, so that a state dict has the reference's keys and shapes, and calls the `kq.*` ops.
@@ -11,6 +12,8 @@ import os
 import torch
 
 from . import ops as kq
+from .lora import _FrozenMatmul, lora_update
+from .moe import gather_lora_update
 
 
 def bytes_per_row(codec: str, dims: int) -> int:
@@ -19,6 +22,12 @@ def bytes_per_row(codec: str, dims: int) -> int:
     if dims % wpb != 0:
         raise ValueError(f"[mlx_kquant] {dims} weights per row is not a whole number of {wpb}-weight {codec} blocks.")
     return dims // wpb * bpb
+
+
+def _dims(layer) -> int:
+    """Weights in a row of a layer's wire bytes."""
+    wpb, bpb, _, _ = kq.codec_geometry(layer.kquant_type)
+    return layer.weight.shape[-1] // bpb * wpb
 
 
 class _KQuantBase(torch.nn.Module):
@@ -162,3 +171,91 @@ class KQuantMultiLinear(_KQuantBase):
     def extra_repr(self) -> str:
         nh, out_dims, bpr = self.weight.shape
         return f"num_heads={nh}, output_dims={out_dims}, bytes_per_row={bpr}, kquant_type={self.kquant_type}"
+
+
+class KQuantLoRALinear(torch.nn.Module):
+    """Low-rank adapters on a `KQuantLinear` (the counterpart of an adapter layer over frozen quantized weights): `lora_a`
+    [n_adapters, rank, in_dims] and `lora_b` [n_adapters, out_dims, rank], zero at first, are its parameters, `scaling` a factor
+    for each adapter. `forward(x, adapter_ids)` gives every row the adapter of its request (`lora_update`); a training step reaches x and
+    the parameters, the wire bytes stay as they are."""
+
+    def __init__(self, base: KQuantLinear, rank: int, n_adapters: int = 1, scaling: float = 1.0, dtype: torch.dtype = torch.float32):
+        super().__init__()
+        out_dims, in_dims = base.weight.shape[0], _dims(base)
+        self.base = base
+        dev = base.weight.device
+        self.lora_a = torch.nn.Parameter((torch.rand(n_adapters, rank, in_dims, device=dev) * 2 - 1).mul_(in_dims ** -0.5).to(dtype))
+        self.lora_b = torch.nn.Parameter(torch.zeros(n_adapters, out_dims, rank, dtype=dtype, device=dev))
+        self.register_buffer("scaling", torch.full((n_adapters,), float(scaling), device=dev))
+
+    def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        base = self.base
+        if torch.is_grad_enabled() and x.requires_grad:
+            y = _FrozenMatmul.apply(x, base.weight, base.scales, base.kquant_type)
+            if base.bias is not None:
+                y = y + base.bias.to(y.dtype)
+        else:
+            y = base(x)
+        return lora_update(y, x, self.lora_a, self.lora_b, adapter_ids, self.scaling)
+
+    def extra_repr(self) -> str:
+        n, r, _ = self.lora_a.shape
+        return f"rank={r}, n_adapters={n}"
+
+
+class _FrozenGather(torch.autograd.Function):
+    """gather_qmm over an expert stack with the gradient of its rows; the wire bytes have none."""
+
+    @staticmethod
+    def forward(ctx, x, w, scales, kquant_type, indices):
+        ctx.kquant_type, ctx.x_shape, ctx.dtype = kquant_type, x.shape, x.dtype
+        ctx.save_for_backward(w, indices)
+        return kq.gather_qmm(x.detach(), w, scales, kquant_type, rhs_indices=indices)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        w, indices = ctx.saved_tensors
+        dx = kq.gather_qmm(dy, w, None, ctx.kquant_type, rhs_indices=indices, transpose=False)
+        there = (indices >= 0) & (indices < w.shape[0])   # rows of other entries are not written
+        dx = torch.where(there[..., None, None], dx.float(), 0.0)
+        return dx.sum_to_size(ctx.x_shape).to(ctx.dtype), None, None, None, None
+
+
+class KQuantLoRASwitchLinear(torch.nn.Module):
+    """Low-rank adapters on a `KQuantSwitchLinear`: a pair of matrices for every adapter and expert, `lora_a` [n_adapters, n_experts,
+    rank, in_dims], `lora_b` [n_adapters, n_experts, out_dims, rank]. `forward(x, indices, adapter_ids, sorted_indices)` takes what the
+    base takes for routed rows: indices [T, R] with x [T, 1, 1, K] (one row per token) or [T, R, 1, K] and adapter_ids [T], or
+    indices [B] with x [B, 1, K] and adapter_ids [B] (`moe.gather_lora_update`)."""
+
+    def __init__(self, base: KQuantSwitchLinear, rank: int, n_adapters: int = 1, scaling: float = 1.0,
+                 dtype: torch.dtype = torch.float32):
+        super().__init__()
+        (n_experts, out_dims, _), in_dims = base.weight.shape, _dims(base)
+        self.base = base
+        dev = base.weight.device
+        self.lora_a = torch.nn.Parameter(
+            (torch.rand(n_adapters, n_experts, rank, in_dims, device=dev) * 2 - 1).mul_(in_dims ** -0.5).to(dtype))
+        self.lora_b = torch.nn.Parameter(torch.zeros(n_adapters, n_experts, out_dims, rank, dtype=dtype, device=dev))
+        self.register_buffer("scaling", torch.full((n_adapters,), float(scaling), device=dev))
+
+    def forward(self, x: torch.Tensor, indices: torch.Tensor, adapter_ids: torch.Tensor | None = None,
+                sorted_indices: bool = False) -> torch.Tensor:
+        base, K = self.base, x.shape[-1]
+        flat = indices.dim() == 1 and x.dim() == 3 and x.shape[:2] == (indices.shape[0], 1)
+        if not flat and not (indices.dim() == 2 and x.dim() == 4 and x.shape[0] == indices.shape[0] and x.shape[2] == 1
+                             and x.shape[1] in (1, indices.shape[1])):
+            raise ValueError(f"KQuantLoRASwitchLinear: x must be [T, 1, 1, K] or [T, R, 1, K] with indices [T, R], or [B, 1, K] with "
+                             f"indices [B], but x is {tuple(x.shape)} and indices {tuple(indices.shape)}.")
+        if torch.is_grad_enabled() and x.requires_grad:
+            y = base._add_bias(_FrozenGather.apply(x, base.weight, base.scales, base.kquant_type, indices), indices)
+        else:
+            y = base(x, indices, sorted_indices)
+        slots = indices.reshape(-1, 1) if flat else indices
+        T, R = slots.shape
+        rows = x.reshape(T, R, K) if flat or x.shape[1] == R else x.reshape(T, K)
+        return gather_lora_update(y.reshape(T, R, -1), rows, self.lora_a, self.lora_b, slots, adapter_ids, self.scaling).reshape(y.shape)
+
+    def extra_repr(self) -> str:
+        n, e, r, _ = self.lora_a.shape
+        return f"rank={r}, n_adapters={n}, n_experts={e}"
