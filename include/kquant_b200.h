@@ -362,9 +362,9 @@ KQ_API int kq_moe_router_grouped_backward(const void* logits, int dtype, long lo
  * expert is outside [0, n_experts) has none: its row of out is y's. f = scale * scaling[adapter] (scaling: float32, or NULL: 1).
  *  kq_lora_update: out[e] = y[e] + f (x[e] . a[g]^T) . b[g]^T; x rows of K values (x_shared != 0: one row per token, else one per
  *    entry), a [n_adapters, n_experts, rank, K], b [n_adapters, n_experts, N, rank], y and out rows of N values; out may be y.
- *    float32 sums, one rounding to out. u: NULL, or float32 [rows, rank] that receives x . a^T (what the gradient needs; zero
- *    for entries without a group).
- *  kq_lora_backward, from dy [rows, N] and that u: dx (rows of x, contiguous in K) = f (dy . b[g]) . a[g], summed over a token's slots
+ *    float32 sums, one rounding to out. saved: NULL, or kq_lora_saved_bytes(rows, rank, param_dtype) bytes, 16-byte aligned, that
+ *    receive x . a^T for the gradient (as bf16 terms: 24 bits of it beside float32 parameters, 16 beside others).
+ *  kq_lora_backward, from dy [rows, N] and that: dx (rows of x, contiguous in K) = f (dy . b[g]) . a[g], summed over a token's slots
  *    where x_shared; da and db, of the parameters' type and shape, whole (zero for groups without entries). Each may be NULL. What
  *    flows to y is dy itself.
  *  dtype: of x, y, out, dy, dx: KQ_F16 or KQ_BF16; param_dtype: of a, b, da, db: the same, or KQ_F32. rank <= 128. Row strides in
@@ -381,13 +381,14 @@ KQ_API int kq_lora_plan(const int32_t* adapter_ids, const uint32_t* experts, lon
 KQ_API int kq_lora_update(const void* x, int dtype, long long rows, int K, long long x_row_stride, int slots, int x_shared,
                           const void* a, const void* b, int param_dtype, int rank, int N, int n_adapters, int n_experts,
                           const int32_t* adapter_ids, const uint32_t* experts, const float* scaling, float scale, const void* y,
-                          long long y_row_stride, void* out, long long out_row_stride, float* u, const void* plan,
+                          long long y_row_stride, void* out, long long out_row_stride, void* saved, const void* plan,
                           size_t plan_bytes, void* stream);
-KQ_API size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int rank);
+KQ_API size_t kq_lora_saved_bytes(long long rows, int rank, int param_dtype);
+KQ_API size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int rank, int param_dtype);
 KQ_API int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long dy_row_stride, const void* x, int K,
                             long long x_row_stride, int slots, int x_shared, const void* a, const void* b, int param_dtype,
                             int rank, int n_adapters, int n_experts, const int32_t* adapter_ids, const uint32_t* experts,
-                            const float* scaling, float scale, const float* u, void* dx, void* da, void* db, const void* plan,
+                            const float* scaling, float scale, const void* saved, void* dx, void* da, void* db, const void* plan,
                             size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

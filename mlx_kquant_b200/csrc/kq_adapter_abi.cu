@@ -138,7 +138,7 @@ int kq_lora_plan(const int32_t* adapter_ids, const uint32_t* experts, long long 
 int kq_lora_update(const void* x, int dtype, long long rows, int K, long long x_row_stride, int slots, int x_shared, const void* a,
                    const void* b, int param_dtype, int rank, int N, int n_adapters, int n_experts, const int32_t* adapter_ids,
                    const uint32_t* experts, const float* scaling, float scale, const void* y, long long y_row_stride, void* out,
-                   long long out_row_stride, float* u, const void* plan, size_t plan_bytes, void* stream) {
+                   long long out_row_stride, void* u, const void* plan, size_t plan_bytes, void* stream) {
   const char* op = "lora_update";
   const int rc = lora_check(op, dtype, param_dtype, rows, K, N, rank, slots, n_adapters, n_experts, adapter_ids, experts, plan, plan_bytes);
   if (rc != KQ_OK || rows == 0) return rc;
@@ -148,13 +148,18 @@ int kq_lora_update(const void* x, int dtype, long long rows, int K, long long x_
   return done(op, kq::launch_lora_forward(c, y, y_row_stride, out, out_row_stride, u, static_cast<cudaStream_t>(stream)));
 }
 
-size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int rank) {
-  return rows < 0 || slots < 1 || K < 1 || rank < 1 ? 0 : kq::lora_backward_workspace_bytes(rows, slots, x_shared, K, rank);
+size_t kq_lora_saved_bytes(long long rows, int rank, int param_dtype) {
+  return rows < 0 || rank < 1 || rank > kq::kLoraMaxRank ? 0 : kq::lora_saved_bytes(rows, rank, param_dtype == KQ_F32);
+}
+
+size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int rank, int param_dtype) {
+  return rows < 0 || slots < 1 || K < 1 || rank < 1 || rank > kq::kLoraMaxRank
+             ? 0 : kq::lora_backward_workspace_bytes(rows, slots, x_shared, K, rank, param_dtype == KQ_F32);
 }
 
 int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long dy_row_stride, const void* x, int K, long long x_row_stride,
                      int slots, int x_shared, const void* a, const void* b, int param_dtype, int rank, int n_adapters, int n_experts,
-                     const int32_t* adapter_ids, const uint32_t* experts, const float* scaling, float scale, const float* u, void* dx,
+                     const int32_t* adapter_ids, const uint32_t* experts, const float* scaling, float scale, const void* u, void* dx,
                      void* da, void* db, const void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   const char* op = "lora_backward";
   const int rc = lora_check(op, dtype, param_dtype, rows, K, N, rank, slots, n_adapters, n_experts, adapter_ids, experts, plan, plan_bytes);
@@ -171,7 +176,7 @@ int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long
   if (!dy || !a || !b || (da && !x) || (db && !u)) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] null pointer.", op);
   if ((adapter_ids != nullptr || experts != nullptr) && plan == nullptr)
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] needs the plan of its indices.", op);
-  if (workspace == nullptr || workspace_bytes < kq_lora_backward_workspace_bytes(rows, slots, x_shared, K, rank))
+  if (workspace == nullptr || workspace_bytes < kq_lora_backward_workspace_bytes(rows, slots, x_shared, K, rank, param_dtype))
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] workspace is smaller than kq_lora_backward_workspace_bytes.", op);
   const kq::LoraCall c{types_of(dtype, param_dtype), kq::LoraGroups{adapter_ids, experts, slots, n_adapters, n_experts, rows, scaling, scale},
                        x, x_row_stride, x_shared, K, N, rank, a, b, plan};

@@ -9,213 +9,254 @@ namespace lora {
 namespace {
 
 // ---------------------------------------------------------------------------------------------------- plan
-constexpr int kPlanThreads = 512, kPlanEach = 8;
+constexpr int kPlanThreads = 512;
 
 // One CTA per group, the last for the entries without one. It reads every entry's group: how many lie before its own, and its
-// own in their order. No counters, nothing to clear, the same order each time. Tiles take the list's slots from
-// start / height + group on, which no two groups share; slots that are left over hold none.
+// own in their order. No counters, nothing to clear, the same order each time. A thread has a run of neighbouring entries, so that
+// one scan over the threads' counts places all of them. Tiles take the list's slots from start / height + group on, which no two
+// groups share; slots that are left over hold none.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const LoraGroups g, int n_groups, int height, int* order, int* offsets, LoraTile* tiles) {
   __shared__ int s_warp[2][kPlanThreads / 32];
-  __shared__ int s_base;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mine = blockIdx.x;
-  const int n = (int)g.n;
-  auto key = [&](int e) {
-    const int k = group_of(g, e);
-    return k < 0 ? n_groups : k;
+  const int n = (int)g.n, each = ((n + kPlanThreads - 1) / kPlanThreads + 3) / 4 * 4;
+  const int e0 = min(n, tid * each), e1 = min(n, e0 + each);
+  // calls f(entry, key) for the thread's entries in order
+  auto walk = [&](auto f) {
+    int token = e0 / g.slots, slot = e0 - token * g.slots;
+    for (int e = e0; e < e1; e += 4) {
+      uint32_t x[4] = {0, 0, 0, 0};
+      if (g.experts != nullptr) {
+        if (e + 4 <= e1 && (reinterpret_cast<uintptr_t>(g.experts) & 15) == 0) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(g.experts + e));
+          x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+          for (int k = 0; k < 4 && e + k < e1; k++) x[k] = g.experts[e + k];
+        }
+      }
+      int id[4] = {0, 0, 0, 0};
+      if (g.ids != nullptr) {
+        if (g.slots == 1 && e + 4 <= e1 && (reinterpret_cast<uintptr_t>(g.ids) & 15) == 0) {
+          const int4 v = __ldg(reinterpret_cast<const int4*>(g.ids + e));
+          id[0] = v.x; id[1] = v.y; id[2] = v.z; id[3] = v.w;
+          token += 4;
+        } else {
+          for (int k = 0; k < 4 && e + k < e1; k++) {
+            id[k] = g.ids[token];
+            if (++slot == g.slots) {
+              slot = 0;
+              token++;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (e + k < e1) f(e + k, (unsigned)id[k] < (unsigned)g.G && x[k] < (uint32_t)g.E ? id[k] * g.E + (int)x[k] : n_groups);
+    }
   };
   int less = 0, same = 0;
-  for (int e = tid; e < n; e += kPlanThreads) {
-    const int k = key(e);
+  walk([&](int, int k) {
     less += k < mine;
     same += k == mine;
-  }
+  });
+  int upto = same;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    less += __shfl_xor_sync(0xffffffffu, less, o);
-    same += __shfl_xor_sync(0xffffffffu, same, o);
+  for (int o = 16; o > 0; o >>= 1) less += __shfl_xor_sync(0xffffffffu, less, o);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
-  if (lane == 0) {
+  if (lane == 31) {
     s_warp[0][warp] = less;
-    s_warp[1][warp] = same;
+    s_warp[1][warp] = upto;
   }
   __syncthreads();
-  int start = 0, count = 0;
+  int start = 0, count = 0, ahead = 0;
+#pragma unroll
   for (int w = 0; w < kPlanThreads / 32; w++) {
+    const int v = s_warp[1][w];
     start += s_warp[0][w];
-    count += s_warp[1][w];
+    if (w < warp) ahead += v;
+    count += v;
   }
   if (tid == 0) {
     offsets[mine] = start;
     if (mine == n_groups) offsets[mine + 1] = start + count;
-    s_base = start;
   }
   // tiles as even as sixteen rows allow
   const int first = start / height + mine, slots = (start + count) / height + mine + 1 - first;
   const int n_tiles = (count + height - 1) / height;
-  const int each = n_tiles > 0 ? ((count + n_tiles - 1) / n_tiles + 15) / 16 * 16 : 0;
+  const int rows = n_tiles > 0 ? ((count + n_tiles - 1) / n_tiles + 15) / 16 * 16 : 0;
   for (int s = tid; s < slots; s += kPlanThreads) {
-    const int at = s * each;
-    tiles[first + s] = LoraTile{mine == n_groups ? -1 : mine, start + at, s < n_tiles ? max(0, min(each, count - at)) : 0, 0};
+    const int at = s * rows;
+    tiles[first + s] = LoraTile{mine == n_groups ? -1 : mine, start + at, s < n_tiles ? max(0, min(rows, count - at)) : 0, 0};
   }
-  if (count == 0) return;
-  for (int e0 = 0; e0 < n; e0 += kPlanThreads * kPlanEach) {
-    __syncthreads();
-    const int base = s_base;
-    uint32_t hits = 0;
-#pragma unroll
-    for (int v = 0; v < kPlanEach; v++) {
-      const int e = e0 + tid * kPlanEach + v;
-      if (e < n && key(e) == mine) hits |= 1u << v;
-    }
-    const int c = __popc(hits);
-    int at = c;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, at, o);
-      if (lane >= o) at += v;
-    }
-    if (lane == 31) s_warp[0][warp] = at;
-    __syncthreads();
-    int ahead = 0, total = 0;
-    for (int w = 0; w < kPlanThreads / 32; w++) {
-      const int v = s_warp[0][w];
-      if (w < warp) ahead += v;
-      total += v;
-    }
-    at += base + ahead - c;
-#pragma unroll
-    for (int v = 0; v < kPlanEach; v++)
-      if (hits >> v & 1) order[at++] = e0 + tid * kPlanEach + v;
-    if (tid == 0) s_base = base + total;   // (read again behind the barrier at the top)
-  }
+  if (same == 0) return;
+  int at = start + ahead + upto - same;
+  walk([&](int e, int k) {
+    if (k == mine) order[at++] = e;
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------- gradients of the matrices
-// A warp's tile: 64 columns of `in` x 16 RT ranks, over the group's entries in sixteens. `in`'s fragments come straight from
-// memory: a lane holds eight neighbouring columns of four entries. Both operands as bf16 terms: fp16 rows are two, exactly; uv is
-// three where the gradient is float32, two where it is rounded to 16 bits. `splits` warps share a tile's entries, and the CTAs of a
-// cluster; their sums meet in a fixed order.
-template <typename XT, typename PT, int RT, bool VEC>
+// A CTA's tile: 128 columns of `in` x 16 RT ranks, over the group's entries in stages of 64. Rows and the terms of u (or v) come by
+// asynchronous copies into a ring; both fragments are transposed on the way out of it (the contraction runs over the entries). Four
+// warps have 32 columns each, the other four the same columns and the other half of a stage's entries. fp16 rows are two bf16
+// terms, exactly. The CTAs of a cluster share a group's stages; all sums meet in a fixed order.
+template <typename PT, int RT>
+struct WgradShape {
+  static constexpr int RP = 16 * RT, UN = sizeof(PT) == 4 ? 3 : 2, ROWS = 64, COLS = 128;
+  static constexpr int IN = ROWS * COLS * 2, UV = ROWS * RP * 2, STAGE = IN + UN * UV;
+  static constexpr int STAGES = 96 * 1024 / STAGE > 5 ? 5 : 96 * 1024 / STAGE < 3 ? 3 : 96 * 1024 / STAGE;
+  static constexpr int OUT = COLS * RP * 4;   // sums of a half of the warps, then of the CTA: in the ring's room
+  static constexpr int SMEM = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+};
+template <typename XT, typename PT, int RT>
 __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) {
-  constexpr int XN = RowTerms<XT, bf16>::N, UN = sizeof(PT) == 4 ? 3 : 2, MOST = UN, JV = 2 * RT, RP = 16 * RT;
-  extern __shared__ float w_smem[];   // [tiles][splits / 2][2 RP][32 lanes] and [tiles][64][RP]
+  typedef WgradShape<PT, RT> S;
+  constexpr int XN = RowTerms<XT, bf16>::N, UN = S::UN, RP = S::RP;
+  typedef Tile<S::COLS, 2> InTile;
+  typedef Tile<RP, 2> UvTile;
+  extern __shared__ __align__(16) uint8_t smem[];
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, q = lane & 3;
-  const int S = a.splits, tiles = kThreads / 32 / S, ct = warp / S, sp = warp % S;
-  const int group = blockIdx.y, j0 = blockIdx.z * 64;
-  const int c0 = (blockIdx.x / C * tiles + ct) * 64;
-  long long start = 0, count = a.g.n;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, q = lane & 3, cq = warp & 3, half = warp >> 2;
+  const int group = blockIdx.y, j0 = blockIdx.z * 64, c0 = blockIdx.x / C * S::COLS;
+  int start = 0, count = (int)a.g.n;
   if (a.offsets != nullptr) {
     start = a.offsets[group];
     count = a.offsets[group + 1] - start;
   }
-  float acc[4][2 * RT][4];
+  const int blocks = (count + S::ROWS - 1) / S::ROWS;
+  const int b0 = (int)((long long)blocks * rank / C), nb = (int)((long long)blocks * (rank + 1) / C) - b0;
+  const uint32_t ring = smem_at(smem);
+  auto fetch = [&](int s) {
+    if (s < nb) {
+      const uint32_t at = ring + s % S::STAGES * S::STAGE;
+      const int t0 = (b0 + s) * S::ROWS;
 #pragma unroll
-  for (int m = 0; m < 4; m++)
+      for (int c = tid; c < S::ROWS * InTile::CHUNKS; c += kThreads) {
+        const int m = c / InTile::CHUNKS, ch = c % InTile::CHUNKS, t = t0 + m;
+        int e = t >= count ? -1 : a.order != nullptr ? a.order[start + t] : t;
+        const int row = e < 0 ? 0 : a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div);
+        load_chunk<2>(InTile::at(at, m, ch), static_cast<const XT*>(a.in) + (long long)row * a.in_stride, c0 + 8 * ch, e < 0 ? 0 : a.D, a.by_in);
+      }
+#pragma unroll
+      for (int c = tid; c < UN * S::ROWS * UvTile::CHUNKS; c += kThreads) {
+        const int n = c / (S::ROWS * UvTile::CHUNKS), m = c / UvTile::CHUNKS % S::ROWS, ch = c % UvTile::CHUNKS, t = t0 + m;
+        const int e = t >= count ? -1 : a.order != nullptr ? a.order[start + t] : t;
+        load_chunk<2>(UvTile::at(at + S::IN + n * S::UV, m, ch), a.uv + ((long long)n * a.g.n + max(e, 0)) * a.ru, j0 + 8 * ch, e < 0 ? 0 : a.ru, kBy16);
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S::STAGES - 1; s++) fetch(s);
+  float acc[2][2 * RT][4];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
 #pragma unroll
     for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
       for (int k = 0; k < 4; k++) acc[m][n][k] = 0.f;
-  if (c0 < a.D) {
-    const int col = c0 + 8 * i;
-    for (long long t0 = 16LL * (rank * S + sp); t0 < count; t0 += 16LL * S * C) {
-      Load<XT, 8, VEC> x[4];
-      float u[4][JV];
+  for (int s = 0; s < nb; s++) {
+    cp_wait<S::STAGES - 2>();
+    __syncthreads();
+    fetch(s + S::STAGES - 1);
+    const uint32_t at = ring + s % S::STAGES * S::STAGE;
+    const int left = count - (b0 + s) * S::ROWS;
+    float part[2][2 * RT][4];   // (a stage's sums by themselves: see the tile kernel)
+    if constexpr (sizeof(PT) == 4) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const long long t = t0 + 4 * q + k;
-        const long long e = t >= count ? -1 : a.order != nullptr ? a.order[start + t] : t;
-        x[k].get(static_cast<const XT*>(a.in) + (e < 0 ? 0 : e / a.in_div) * a.in_stride + col, e < 0 ? 0 : a.D - col);
-        const float* up = a.uv + (e < 0 ? 0 : e) * a.r + j0 + i * JV;
+      for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int j = 0; j < JV; j++) u[k][j] = e >= 0 && j0 + i * JV + j < a.r ? up[j] : 0.f;
+        for (int n = 0; n < 2 * RT; n++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) part[m][n][k] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int t = 16 * (2 * k + half);
+      if (t >= left) continue;
+      uint32_t xa[2][XN][4];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        uint32_t raw[4];
+        ldsm_trans(raw, InTile::at(at, t + (lane & 7) + ((lane >> 4) & 1) * 8, 4 * cq + 2 * m + ((lane >> 3) & 1)));
+        RowTerms<XT, bf16>::get(raw, xa[m]);
       }
-      uint32_t xa[4][XN][4];
 #pragma unroll
-      for (int m = 0; m < 4; m++) {
-        const uint32_t p[4] = {__byte_perm(x[0].w[m], x[1].w[m], 0x5410), __byte_perm(x[0].w[m], x[1].w[m], 0x7632),
-                               __byte_perm(x[2].w[m], x[3].w[m], 0x5410), __byte_perm(x[2].w[m], x[3].w[m], 0x7632)};
+      for (int n = 0; n < RT; n++) {
+        uint32_t b[2][2][UN];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          uint32_t t[XN];
-          RowTerms<XT, bf16>::get(p[k], t);
-#pragma unroll
-          for (int n = 0; n < XN; n++) xa[m][n][k] = t[n];
+        for (int u = 0; u < UN; u++) {
+          uint32_t r[4];
+          ldsm_trans(r, UvTile::at(at + S::IN + u * S::UV, t + (lane & 15), 2 * n + (lane >> 4)));
+          b[0][0][u] = r[0]; b[0][1][u] = r[1]; b[1][0][u] = r[2]; b[1][1][u] = r[3];
         }
-      }
 #pragma unroll
-      for (int jt = 0; jt < 2 * RT; jt++) {
-        uint32_t b0[UN], b1[UN];
-        split<UN>(u[0][jt], u[1][jt], b0);
-        split<UN>(u[2][jt], u[3][jt], b1);
+        for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int m = 0; m < 4; m++) mma_terms<XN, UN, MOST, bf16>(acc[m][jt], xa[m], b0, b1);
+          for (int h = 0; h < 2; h++) {
+            if constexpr (sizeof(PT) == 4) mma_terms<XN, UN, bf16>(part[m][2 * n + h], xa[m], b[h][0], b[h][1]);
+            else mma_terms<XN, UN, bf16>(acc[m][2 * n + h], xa[m], b[h][0], b[h][1]);
+          }
       }
     }
-  }
-  for (int h = S / 2; h > 0; h >>= 1) {
-    float* mine = w_smem + (size_t)(ct * (S / 2) + sp % h) * 2 * RP * 16 * 2;
-    if (sp >= h && sp < 2 * h) {
+    if constexpr (sizeof(PT) == 4) {
 #pragma unroll
-      for (int m = 0; m < 4; m++)
+      for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) mine[((m * 2 * RT + n) * 4 + k) * 32 + lane] = acc[m][n][k];
+          for (int k = 0; k < 4; k++) acc[m][n][k] += part[m][n][k];
     }
-    __syncthreads();
-    if (sp < h) {
+  }
+  cp_wait<0>();
+  __syncthreads();
+  // [columns][ranks] in shared memory: one half of the warps, then both; the CTAs of the cluster add and store a part of it each
+  float* s_out = reinterpret_cast<float*>(smem);
 #pragma unroll
-      for (int m = 0; m < 4; m++)
+  for (int turn = 1; turn >= 0; turn--) {
+    if (half == turn) {
+#pragma unroll
+      for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) acc[m][n][k] += mine[((m * 2 * RT + n) * 4 + k) * 32 + lane];
+          for (int k = 0; k < 4; k++) {
+            float* o = s_out + (32 * cq + 16 * m + i + 8 * (k >> 1)) * RP + 8 * n + 2 * q + (k & 1);
+            *o = turn == 1 ? acc[m][n][k] : *o + acc[m][n][k];
+          }
     }
     __syncthreads();
   }
-  // [64 columns][RP ranks] of each tile in shared memory; the CTAs of the cluster add and store a part of it each
-  float* s_out = w_smem + (size_t)tiles * (S / 2) * 64 * RP;
-  if (sp == 0) {
-#pragma unroll
-    for (int m = 0; m < 4; m++)
-#pragma unroll
-      for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          s_out[(ct * 64 + 8 * i + 2 * m + (k >> 1)) * RP + (2 * q + (k & 1)) * JV + n] = acc[m][n][k];
-  }
-  cluster.sync();
+  if (C > 1) cluster.sync();
   const float f = a.scaled ? factor_of(a.g, group) : 1.f;
-  const int r1 = min(RP, a.r - j0);
+  const int r1 = min(RP, a.r - j0), cols = min(S::COLS, a.D - c0);
   PT* out = static_cast<PT*>(a.out) + (long long)group * a.r * a.D;
-  const int per = tiles * 64 * r1;
-  for (int v = rank * kThreads + tid; v < per; v += C * kThreads) {
-    const int c = a.r_first ? v % (tiles * 64) : v / r1, j = a.r_first ? v / (tiles * 64) : v % r1;
-    const long long column = (long long)blockIdx.x / C * tiles * 64 + c;
-    if (column >= a.D) continue;
+  for (int v = rank * kThreads + tid; v < cols * r1; v += C * kThreads) {
+    const int c = a.r_first ? v % cols : v / r1, j = a.r_first ? v / cols : v % r1;
     float s = 0.f;
-    for (int b = 0; b < C; b++) s += *cluster.map_shared_rank(s_out + c * RP + j, b);
-    out[a.r_first ? (long long)(j0 + j) * a.D + column : column * a.r + j0 + j] = PT(s * f);
+    if (C == 1) s = s_out[c * RP + j];
+    else
+      for (int b = 0; b < C; b++) s += *cluster.map_shared_rank(s_out + c * RP + j, b);
+    out[a.r_first ? (long long)(j0 + j) * a.D + c0 + c : (long long)(c0 + c) * a.r + j0 + j] = PT(s * f);
   }
-  cluster.sync();
+  if (C > 1) cluster.sync();
 }
 
-template <typename XT, typename PT, int RT, bool VEC>
+template <typename XT, typename PT, int RT>
 cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
-  constexpr int RP = 16 * RT;
-  const int tiles = kThreads / 32 / a.splits;
-  const int smem = (tiles * (a.splits / 2) + tiles) * 64 * RP * 4;
-  auto kern = wgrad_kernel<XT, PT, RT, VEC>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * 64 * RP * 4);
-    if (e != cudaSuccess) return e;
-  }
+  typedef WgradShape<PT, RT> S;
+  auto kern = wgrad_kernel<XT, PT, RT>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.D + 64 * tiles - 1) / (64 * tiles) * cluster), (unsigned)a.n_groups, (unsigned)((a.r + 63) / 64));
+  cfg.gridDim = dim3((unsigned)((a.D + S::COLS - 1) / S::COLS * cluster), (unsigned)a.n_groups, (unsigned)((a.r + 63) / 64));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -226,14 +267,9 @@ cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
 }
 template <typename XT, typename PT>
 cudaError_t wgrad_rank(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
-  if (a.vec_in) {
-    if (a.r <= 16) return wgrad_launch<XT, PT, 1, true>(a, cluster, st);
-    if (a.r <= 32) return wgrad_launch<XT, PT, 2, true>(a, cluster, st);
-    return wgrad_launch<XT, PT, 4, true>(a, cluster, st);
-  }
-  if (a.r <= 16) return wgrad_launch<XT, PT, 1, false>(a, cluster, st);
-  if (a.r <= 32) return wgrad_launch<XT, PT, 2, false>(a, cluster, st);
-  return wgrad_launch<XT, PT, 4, false>(a, cluster, st);
+  if (a.r <= 16) return wgrad_launch<XT, PT, 1>(a, cluster, st);
+  if (a.r <= 32) return wgrad_launch<XT, PT, 2>(a, cluster, st);
+  return wgrad_launch<XT, PT, 4>(a, cluster, st);
 }
 
 // ---------------------------------------------------------------------------------------------------- sum over slots
@@ -246,8 +282,6 @@ __global__ void __launch_bounds__(kThreads) sum_slots_kernel(const float* part, 
     out[token * out_stride + c] = XT(s);
   }
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int sm_count() {
   int dev = 0, sms = 0;
@@ -300,13 +334,20 @@ int set_rows(LoraArgs& a, const LoraCall& c, int& cluster) {
   return mt;
 }
 
-void set_vec(LoraArgs& a, const LoraCall& c, bool backward) {
-  const int rt = a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8;
-  a.vec_in = a.D1 % 8 == 0 && a.in_stride % 8 == 0 && aligned16(a.in);
-  a.vec_w1 = aligned16(a.w1) && (backward ? a.r % (2 * rt) == 0 : a.D1 % 8 == 0);
-  a.vec_w2 = aligned16(a.w2) && (backward ? a.D2 % 8 == 0 : a.r % 4 == 0);
-  a.vec_out = a.D2 % 8 == 0 && a.out_stride % 8 == 0 && aligned16(a.out) &&
-              (a.base == nullptr || (a.base_stride % 8 == 0 && aligned16(a.base)));
+// how rows of `size`-byte elements, `stride` apart from `p` on, of `length` elements, can be read
+int by(const void* p, long long stride, int length, int size) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * size) | (uintptr_t)((long long)length * size);
+  return (all & 15) == 0 ? kBy16 : (all & 7) == 0 ? kBy8 : kByElement;
+}
+
+void set_reads(LoraArgs& a, const LoraCall& c, bool backward) {
+  const int ps = c.types == kLoraBf16 || c.types == kLoraF16 ? 2 : 4;
+  const int l1 = backward ? a.r : a.D1, l2 = backward ? a.D2 : a.r;
+  a.by_in = by(a.in, a.in_stride, a.D1, 2);
+  a.by_w1 = by(a.w1, l1, l1, ps);
+  a.by_w2 = by(a.w2, l2, l2, ps);
+  a.vec_out = by(a.out, a.out_stride, a.D2, 2) == kBy16 && (a.base == nullptr || by(a.base, a.base_stride, a.D2, 2) == kBy16);
+  a.ru = (a.r + 7) / 8 * 8;
 }
 
 }  // namespace
@@ -347,7 +388,7 @@ cudaError_t launch_lora_sum_slots(const float* part, int slots, long long tokens
   return cudaGetLastError();
 }
 
-cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_stride, void* out, long long out_stride, float* u,
+cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_stride, void* out, long long out_stride, void* u,
                                 cudaStream_t st) {
   LoraArgs a{};
   int cluster;
@@ -365,9 +406,9 @@ cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_st
   a.out = out;
   a.out_stride = out_stride;
   a.c1 = c.N;
-  a.u = u;
+  a.u = static_cast<uint16_t*>(u);
   a.shrink = 1;
-  set_vec(a, c, false);
+  set_reads(a, c, false);
   return tile_launch(c.types, a, false, mt, cluster, st);
 }
 
@@ -376,18 +417,20 @@ static int slot_columns(long long n, int K) {
   const long long fit = (long long)(kSlotBytes / 4) / std::max<long long>(1, n) / 64 * 64;
   return (int)std::min<long long>(K, std::max<long long>(64, fit));
 }
-static size_t v_bytes(long long n, int r) { return ((size_t)n * r * 4 + 255) & ~(size_t)255; }
-size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int r) {
-  return v_bytes(n, r) + (shared && slots > 1 ? (size_t)n * slot_columns(n, K) * 4 : 0);
+size_t lora_saved_bytes(long long n, int r, int param_f32) { return (size_t)n * ((r + 7) / 8 * 8) * (param_f32 ? 6 : 4); }
+static size_t v_bytes(long long n, int r, int f32) { return (lora_saved_bytes(n, r, f32) + 255) & ~(size_t)255; }
+size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int r, int param_f32) {
+  return v_bytes(n, r, param_f32) + (shared && slots > 1 ? (size_t)n * slot_columns(n, K) * 4 : 0);
 }
 
-cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy_stride, const float* u, void* dx, long long dx_stride,
+cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy_stride, const void* u, void* dx, long long dx_stride,
                                  void* da, void* db, void* workspace, cudaStream_t st) {
   LoraArgs a{};
   cudaError_t e;
   int cluster;
   const bool summed = c.shared && c.g.slots > 1;
-  float* v = static_cast<float*>(workspace);
+  const int f16 = c.types == kLoraF16 || c.types == kLoraF16F32, f32 = c.types == kLoraBf16F32 || c.types == kLoraF16F32;
+  uint16_t* v = static_cast<uint16_t*>(workspace);
   a.r = c.r;
   const int mt = set_rows(a, c, cluster);
   a.in = dy;
@@ -405,14 +448,13 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
     a.out = dx;
     a.out_stride = dx_stride;
   }
-  set_vec(a, c, true);
+  set_reads(a, c, true);
   if (dx != nullptr || da != nullptr) {
     if ((e = tile_launch(c.types, a, true, mt, cluster, st)) != cudaSuccess) return e;
   }
-  const int f16 = c.types == kLoraF16 || c.types == kLoraF16F32, f32 = c.types == kLoraBf16F32 || c.types == kLoraF16F32;
   if (dx != nullptr && summed) {
     const long long tokens = c.g.n / c.g.slots;
-    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(c.g.n, c.r));
+    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(c.g.n, c.r, f32));
     const int step = slot_columns(c.g.n, c.K);
     a.shrink = 0;
     a.out = part;
@@ -421,7 +463,7 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
       a.c0 = c0;
       a.c1 = std::min(c.K, c0 + step);
       a.out_stride = a.c1 - a.c0;
-      set_vec(a, c, true);
+      set_reads(a, c, true);
       if ((e = tile_launch(c.types, a, true, mt, cluster, st)) != cudaSuccess) return e;
       if ((e = launch_lora_sum_slots(part, c.g.slots, tokens, a.c1 - a.c0, static_cast<uint16_t*>(dx) + c0, dx_stride, f16 ? 1 : 2, st)) !=
           cudaSuccess)
@@ -434,21 +476,22 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
   w.n_groups = c.g.G * c.g.E;
   w.order = a.plan.order;
   w.offsets = a.plan.offsets;
-  // few entries of a group: its warps take columns of their own; many: they share the entries, and the CTAs of a cluster
-  const long long rows = c.g.n / w.n_groups;
-  w.splits = rows >= 512 ? 8 : rows >= 128 ? 2 : 1;
-  auto wgrad = [&](const void* in, long long stride, int div, int D, const float* uv, int scaled, void* out, int r_first) {
+  w.ru = a.ru;
+  // CTAs of a cluster share a group's stages of 64 entries, where the columns alone leave the GPU empty
+  const long long stages = (c.g.n / w.n_groups + 63) / 64;
+  auto wgrad = [&](const void* in, long long stride, int div, int D, const void* uv, int scaled, void* out, int r_first) {
     w.in = in;
     w.in_stride = stride;
     w.in_div = div;
     w.D = D;
-    w.uv = uv;
+    w.uv = static_cast<const uint16_t*>(uv);
     w.scaled = scaled;
     w.out = out;
     w.r_first = r_first;
-    w.vec_in = D % 8 == 0 && stride % 8 == 0 && aligned16(in);
-    const long long ctas = (long long)w.n_groups * ((D + 64 * (8 / w.splits) - 1) / (64 * (8 / w.splits)));
-    return launch_lora_wgrad(w, f16 ? 1 : 2, f32, rows >= 512 ? pick_cluster(ctas) : 1, st);
+    w.by_in = by(in, stride, D, 2);
+    int cluster = pick_cluster((long long)w.n_groups * ((D + 127) / 128));
+    while (cluster > 1 && stages < 2 * cluster) cluster >>= 1;
+    return launch_lora_wgrad(w, f16 ? 1 : 2, f32, cluster, st);
   };
   if (db != nullptr && (e = wgrad(dy, dy_stride, 1, c.N, u, 1, db, 0)) != cudaSuccess) return e;
   if (da != nullptr && (e = wgrad(c.x, c.x_stride, c.shared ? c.g.slots : 1, c.K, v, 0, da, 1)) != cudaSuccess) return e;

@@ -1,14 +1,16 @@
 // Low-rank adapters beside a shared projection: the kernel of both products, in . w1^T -> u and base + f u . w2^T -> out.
 //
-// A cluster of CTAs takes a tile of rows that share an adapter. Each CTA multiplies a part of the contraction, the parts of u
-// meet over distributed shared memory in the order of the CTAs, and each CTA makes a part of the output's columns: one launch,
-// rows read once, outputs written once, the adapter's matrices read once per tile. The products are mma.sync m16n8k16: a tile's
-// work is bound by its bytes, and the fragments come straight from global memory, 16 bytes a lane, under a permutation of the
-// contraction (both operands alike) or of the output's columns that makes a lane's share contiguous.
+// A cluster of CTAs takes a tile of 16 or 64 rows that share an adapter. Each CTA multiplies a part of the contraction, the parts of
+// u meet over distributed shared memory in the order of the CTAs, and each CTA makes a part of the output's columns: one launch,
+// rows read once, outputs written once, the adapter's matrices read once per tile. Rows and weights of both products pass through
+// one ring of stages in shared memory, filled by 16-byte asynchronous copies (the rows of a tile lie anywhere), so that the second
+// product's weights and the base's rows are on their way while the first ends. The products are mma.sync m16n8k16 on ldmatrix
+// fragments, sums in float32.
 //
-// float32 parameters are split into bf16 terms of 8 bits: three where the result is kept in float32 (u), two where it is rounded to
-// 16 bits; fp16 rows are then two bf16 terms, exactly. u enters the second product as two terms of the row's type, fp16 ones
-// under a power of two per row.
+// float32 parameters are split into bf16 terms of 8 bits as they are read from shared memory: three where the result is kept in
+// float32 (u), two where it is rounded to 16 bits; fp16 rows are then two bf16 terms, exactly. u enters the second product as two
+// terms of the row's type, fp16 ones under a power of two per row. It is saved for the gradients as three bf16 terms beside float32
+// parameters, as two beside 16-bit ones, whose gradients are rounded to 16 bits.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -45,9 +47,7 @@ __device__ __forceinline__ float factor_of(const LoraGroups& g, int group) {
 }
 
 // ---------------------------------------------------------------------------------------------------- fragments
-__device__ __forceinline__ uint32_t pack(bf16 lo, bf16 hi) {
-  return (uint32_t)__bfloat16_as_ushort(lo) | (uint32_t)__bfloat16_as_ushort(hi) << 16;
-}
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bf16) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -58,19 +58,27 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The leading bits of two floats as a bf16 pair, cut off (never rounded up to infinity), and what is left of them.
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t round_bf16(float f0, float f1) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(f0, f1);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// The leading bits of two floats as a bf16 pair, cut off (never rounded up to infinity), and what is left of them: of an infinity
+// nothing.
 __device__ __forceinline__ uint32_t take_bf16(float& f0, float& f1) {
   const uint32_t b0 = __float_as_uint(f0) & 0xffff0000u, b1 = __float_as_uint(f1) & 0xffff0000u;
-  // nothing is left of an infinity; a NaN whose bits all lie below stays one in the rest
   f0 = fabsf(f0) == INFINITY ? 0.f : f0 - __uint_as_float(b0);
   f1 = fabsf(f1) == INFINITY ? 0.f : f1 - __uint_as_float(b1);
   return __byte_perm(b0, b1, 0x7632);
 }
-__device__ __forceinline__ uint32_t round_bf16(float f0, float f1) {
-  return pack(__float2bfloat16_rn(f0), __float2bfloat16_rn(f1));
-}
-
-// N terms of the pair (f0, f1).
+// N bf16 terms of the pair (f0, f1)
 template <int N>
 __device__ __forceinline__ void split(float f0, float f1, uint32_t (&t)[N]) {
 #pragma unroll
@@ -82,68 +90,26 @@ __device__ __forceinline__ void split(float f0, float f1, uint32_t (&t)[N]) {
 template <typename XT, typename CT>
 struct RowTerms {
   static constexpr int N = std::is_same<XT, CT>::value ? 1 : 2;
-  __device__ static __forceinline__ void get(uint32_t v, uint32_t (&t)[N]) {
-    if constexpr (N == 1) {
-      t[0] = v;
-    } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-      split<2>(f.x, f.y, t);
-    }
-  }
-};
-
-// `N` contiguous elements as pairs of words, guarded: elements from `valid` on are zero.
-template <typename T, int N, bool VEC>
-struct Load {
-  static constexpr int WORDS = N * (int)sizeof(T) / 4;
-  uint32_t w[WORDS];
-  __device__ __forceinline__ void zero() {
+  __device__ static __forceinline__ void get(const uint32_t (&v)[4], uint32_t (&t)[N][4]) {
 #pragma unroll
-    for (int i = 0; i < WORDS; i++) w[i] = 0;
-  }
-  __device__ __forceinline__ void get(const T* p, int valid) {
-    if constexpr (VEC) {   // all or nothing
-      if (valid <= 0) { zero(); return; }
-      if constexpr (WORDS >= 4) {
-#pragma unroll
-        for (int i = 0; i < WORDS; i += 4) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
-          w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
-        }
-      } else if constexpr (WORDS == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x; w[1] = v.y;
+    for (int k = 0; k < 4; k++) {
+      if constexpr (N == 1) {
+        t[0][k] = v[k];
       } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+        uint32_t p[2];
+        split<2>(f.x, f.y, p);
+        t[0][k] = p[0];
+        t[1][k] = p[1];
       }
-    } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < N; i++) w[i] = i < valid ? __float_as_uint((float)p[i]) : 0u;
-    } else {
-      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-      for (int i = 0; i < N / 2; i++)
-        w[i] = (2 * i < valid ? (uint32_t)h[2 * i] : 0u) | (2 * i + 1 < valid ? (uint32_t)h[2 * i + 1] << 16 : 0u);
     }
   }
 };
 
-// the pair (x[i], x[i + 1]) of a load, i even, as terms
-template <typename PT, int TERMS, int N, bool VEC>
-__device__ __forceinline__ void pair_along(const Load<PT, N, VEC>& l, int i, uint32_t (&t)[TERMS]) {
-  if constexpr (sizeof(PT) == 2) t[0] = l.w[i / 2];
-  else split<TERMS>(__uint_as_float(l.w[i]), __uint_as_float(l.w[i + 1]), t);
-}
-// the pair (p[i], q[i]) of two loads
-template <typename PT, int TERMS, int N, bool VEC>
-__device__ __forceinline__ void pair_across(const Load<PT, N, VEC>& p, const Load<PT, N, VEC>& q, int i, uint32_t (&t)[TERMS]) {
-  if constexpr (sizeof(PT) == 2) t[0] = __byte_perm(p.w[i / 2], q.w[i / 2], (i & 1) ? 0x7632 : 0x5410);
-  else split<TERMS>(__uint_as_float(p.w[i]), __uint_as_float(q.w[i]), t);
-}
-
-template <int XN, int PN, int MOST, typename CT>
+// all products of the terms but those below the last one's bits, smallest first
+template <int XN, int PN, typename CT>
 __device__ __forceinline__ void mma_terms(float (&c)[4], const uint32_t (&a)[XN][4], const uint32_t (&b0)[PN], const uint32_t (&b1)[PN]) {
-  // smallest products first; those below the last term's bits are left out
+  constexpr int MOST = PN > XN ? PN : XN;
 #pragma unroll
   for (int s = MOST - 1; s >= 0; s--)
 #pragma unroll
@@ -151,6 +117,89 @@ __device__ __forceinline__ void mma_terms(float (&c)[4], const uint32_t (&a)[XN]
 #pragma unroll
       for (int j = 0; j < PN; j++)
         if (i + j == s) mma(c, a[i], b0[j], b1[j], CT());
+}
+
+// ---------------------------------------------------------------------------------------------------- shared-memory tiles
+// ROWS x COLS elements in chunks of 16 bytes; a row's chunks are permuted so that the eight rows of a matrix fragment, and eight
+// neighbouring chunks of a row, lie in different banks.
+template <int COLS, int ES>
+struct Tile {
+  static constexpr int CHUNKS = COLS * ES / 16, PER = 16 / ES;   // chunks of a row, elements of a chunk
+  __device__ static __forceinline__ int chunk(int row, int c) {
+    if constexpr (CHUNKS >= 8) return row * CHUNKS + (c ^ (row & 7));
+    else return row * CHUNKS + (c ^ ((row / (8 / CHUNKS)) & (CHUNKS - 1)));
+  }
+  __device__ static __forceinline__ uint32_t at(uint32_t base, int row, int c) { return base + 16 * chunk(row, c); }
+};
+
+// how a matrix's rows can be read: 16 bytes at a time, 8, or element by element
+enum { kBy16 = 0, kBy8 = 1, kByElement = 2 };
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+// One chunk: elements [e, e + PER) of a row of which `valid` exist; the others become zero.
+template <int ES>
+__device__ __forceinline__ void load_chunk(uint32_t dst, const void* row, int e, int valid, int by) {
+  constexpr int PER = 16 / ES;
+  const uint8_t* p = static_cast<const uint8_t*>(row) + (long long)e * ES;
+  if (by == kBy16) {
+    cp16(dst, e < valid ? p : row, e < valid);
+  } else if (by == kBy8) {
+    cp8(dst, e < valid ? p : row, e < valid);
+    cp8(dst + 8, e + PER / 2 < valid ? p + 8 : row, e + PER / 2 < valid);
+  } else {
+    uint32_t w[4];
+    if constexpr (ES == 2) {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        w[i] = (e + 2 * i < valid ? (uint32_t)h[2 * i] : 0u) | (e + 2 * i + 1 < valid ? (uint32_t)h[2 * i + 1] << 16 : 0u);
+    } else {
+      const uint32_t* h = reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = e + i < valid ? h[i] : 0u;
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+  }
+}
+
+// Fragments of the second operand for sixteen columns (two n8 tiles) and a k16 step: b[tile][half][term]. ALONG: the tile's rows are
+// the product's columns, the contraction runs along them; otherwise its rows are the contraction.
+template <typename PT, int TERMS, int COLS, bool ALONG>
+__device__ __forceinline__ void load_b(uint32_t base, int col0, int k0, uint32_t (&b)[2][2][TERMS]) {
+  typedef Tile<COLS, sizeof(PT)> W;
+  const int l = threadIdx.x & 31;
+  if constexpr (sizeof(PT) == 2) {
+    uint32_t r[4];
+    if constexpr (ALONG) ldsm(r, W::at(base, col0 + (l & 7) + ((l >> 4) & 1) * 8, k0 / 8 + ((l >> 3) & 1)));
+    else ldsm_trans(r, W::at(base, k0 + (l & 15), col0 / 8 + (l >> 4)));
+    b[0][0][0] = r[0]; b[0][1][0] = r[1]; b[1][0][0] = r[2]; b[1][1][0] = r[3];
+  } else {
+    const int i = l >> 2, q = l & 3;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float f0, f1;
+        if constexpr (ALONG) {
+          const uint32_t p = W::at(base, col0 + 8 * t + i, (k0 + 8 * h) / 4 + (q >> 1)) + 8 * (q & 1);
+          asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(f0), "=f"(f1) : "r"(p) : "memory");
+        } else {
+          const int k = k0 + 8 * h + 2 * q, c = (col0 + 8 * t) / 4 + (i >> 2);
+          asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(f0) : "r"(W::at(base, k, c) + 4 * (i & 3)) : "memory");
+          asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(f1) : "r"(W::at(base, k + 1, c) + 4 * (i & 3)) : "memory");
+        }
+        split<TERMS>(f0, f1, b[t][h]);
+      }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------- tile
@@ -209,36 +258,6 @@ __device__ __forceinline__ TileAt find_tile(const LoraArgs& a, int tile, int* s_
 template <typename XT>
 __device__ __forceinline__ float to_float(XT v) { return static_cast<float>(v); }
 
-// eight neighbouring columns of an output row
-template <typename XT>
-__device__ __forceinline__ void store8(const LoraArgs& a, int row, int col, int c_end, const float (&v)[8], float f) {
-  if (a.out_f32) {
-    float* o = static_cast<float*>(a.out) + (long long)row * a.out_stride + (col - a.c0);
-    if (a.vec_out && col + 8 <= c_end) {
-      reinterpret_cast<float4*>(o)[0] = make_float4(f * v[0], f * v[1], f * v[2], f * v[3]);
-      reinterpret_cast<float4*>(o)[1] = make_float4(f * v[4], f * v[5], f * v[6], f * v[7]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (col + i < c_end) o[i] = f * v[i];
-    }
-    return;
-  }
-  XT* o = static_cast<XT*>(a.out) + (long long)row * a.out_stride + (col - a.c0);
-  const XT* b = static_cast<const XT*>(a.base) + (long long)row * a.base_stride + (col - a.c0);
-  if (a.vec_out && col + 8 <= c_end) {
-    uint4 raw = a.base != nullptr ? *reinterpret_cast<const uint4*>(b) : make_uint4(0, 0, 0, 0);
-    XT* h = reinterpret_cast<XT*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 8; i++) h[i] = XT(fmaf(f, v[i], a.base != nullptr ? to_float(h[i]) : 0.f));
-    *reinterpret_cast<uint4*>(o) = raw;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (col + i < c_end) o[i] = XT(fmaf(f, v[i], a.base != nullptr ? to_float(b[i]) : 0.f));
-  }
-}
-
 // rows without an adapter: the base as it is
 template <typename XT>
 __device__ __forceinline__ void copy_rows(const LoraArgs& a, const int* s_row, int rows, int lo, int hi) {
@@ -252,7 +271,7 @@ __device__ __forceinline__ void copy_rows(const LoraArgs& a, const int* s_row, i
     }
     XT* o = static_cast<XT*>(a.out) + (long long)row * a.out_stride - a.c0;
     const XT* b = static_cast<const XT*>(a.base) + (long long)row * a.base_stride - a.c0;
-    if (a.vec_out && lo % 8 == 0 && hi % 8 == 0) {
+    if (a.vec_out) {
       for (int c = lo + 8 * threadIdx.x; c < hi; c += 8 * kThreads)
         *reinterpret_cast<uint4*>(o + c) = a.base != nullptr ? *reinterpret_cast<const uint4*>(b + c) : make_uint4(0, 0, 0, 0);
     } else {
@@ -261,241 +280,175 @@ __device__ __forceinline__ void copy_rows(const LoraArgs& a, const int* s_row, i
   }
 }
 
-// ---- first product: a warp's part of u, [16 WT rows] x [16 RT ranks], over the 32-blocks k0, k0 + step, ... below k1
-template <typename XT, typename PT, typename CT, bool BWD, int RT, int WT, bool VI, bool VW>
-__device__ __forceinline__ void shrink_part(const LoraArgs& a, const PT* w1, const int* s_row, int m0, int k0, int k1, int step,
-                                            float (&acc)[WT][2 * RT][4]) {
-  constexpr int XN = RowTerms<XT, CT>::N, PN = sizeof(PT) == 4 ? 3 : 1;
-  constexpr int MOST = PN > XN ? PN : XN;
-  constexpr int JV = 2 * RT;
-  const int lane = threadIdx.x & 31, i = lane >> 2, q = lane & 3;
-  const XT* xp[WT][2];
-#pragma unroll
-  for (int m = 0; m < WT; m++)
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int e = s_row[m0 + 16 * m + 8 * h + i];
-      xp[m][h] = e < 0 ? nullptr : static_cast<const XT*>(a.in) + (long long)(a.in_div == 1 ? e : e / a.in_div) * a.in_stride;
-    }
-  for (int k = k0; k < k1; k += step) {
-    const int kk = k + 8 * q;
-    Load<XT, 8, VI> x[WT][2];
-#pragma unroll
-    for (int m = 0; m < WT; m++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) x[m][h].get(xp[m][h] + kk, xp[m][h] == nullptr ? 0 : a.D1 - kk);
-    if constexpr (!BWD) {
-#pragma unroll
-      for (int jt = 0; jt < 2 * RT; jt++) {
-        const int j = 8 * jt + i;
-        Load<PT, 8, VW> w;
-        w.get(w1 + (long long)j * a.D1 + kk, j < a.r ? a.D1 - kk : 0);
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-          uint32_t b0[PN], b1[PN];
-          pair_along<PT, PN>(w, 4 * s, b0);
-          pair_along<PT, PN>(w, 4 * s + 2, b1);
-#pragma unroll
-          for (int m = 0; m < WT; m++) {
-            uint32_t xa[XN][4], t0[XN], t1[XN], t2[XN], t3[XN];
-            RowTerms<XT, CT>::get(x[m][0].w[2 * s], t0);
-            RowTerms<XT, CT>::get(x[m][1].w[2 * s], t1);
-            RowTerms<XT, CT>::get(x[m][0].w[2 * s + 1], t2);
-            RowTerms<XT, CT>::get(x[m][1].w[2 * s + 1], t3);
-#pragma unroll
-            for (int n = 0; n < XN; n++) { xa[n][0] = t0[n]; xa[n][1] = t1[n]; xa[n][2] = t2[n]; xa[n][3] = t3[n]; }
-            mma_terms<XN, PN, MOST, CT>(acc[m][jt], xa, b0, b1);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 2; s++) {
-        uint32_t xa[WT][XN][4];
-#pragma unroll
-        for (int m = 0; m < WT; m++) {
-          uint32_t t0[XN], t1[XN], t2[XN], t3[XN];
-          RowTerms<XT, CT>::get(x[m][0].w[2 * s], t0);
-          RowTerms<XT, CT>::get(x[m][1].w[2 * s], t1);
-          RowTerms<XT, CT>::get(x[m][0].w[2 * s + 1], t2);
-          RowTerms<XT, CT>::get(x[m][1].w[2 * s + 1], t3);
-#pragma unroll
-          for (int n = 0; n < XN; n++) { xa[m][n][0] = t0[n]; xa[m][n][1] = t1[n]; xa[m][n][2] = t2[n]; xa[m][n][3] = t3[n]; }
-        }
-        // rows kk + 4 s .. + 3 of w1, a lane's JV neighbouring ranks of each
-        Load<PT, JV, VW> w[4];
-#pragma unroll
-        for (int n = 0; n < 4; n++) w[n].get(w1 + (long long)(kk + 4 * s + n) * a.r + i * JV, kk + 4 * s + n < a.D1 ? a.r - i * JV : 0);
-#pragma unroll
-        for (int jt = 0; jt < 2 * RT; jt++) {
-          uint32_t b0[PN], b1[PN];
-          pair_across<PT, PN>(w[0], w[1], jt, b0);
-          pair_across<PT, PN>(w[2], w[3], jt, b1);
-#pragma unroll
-          for (int m = 0; m < WT; m++) mma_terms<XN, PN, MOST, CT>(acc[m][jt], xa[m], b0, b1);
-        }
-      }
-    }
-  }
-}
-
-// ---- second product: the CTA's columns [lo, hi), a warp a chunk of 32 (forward) or 64 (backward) after another
-template <typename XT, typename PT, typename CT, bool BWD, int RT, int MT, bool VW>
-__device__ __forceinline__ void expand_part(const LoraArgs& a, const PT* w2, const int* s_row, const float* s_factor, const uint16_t* s_u,
-                                            int rows, int lo, int hi) {
-  constexpr int PN = sizeof(PT) == 4 ? 2 : 1, UP = 16 * RT + 8, CH = BWD ? 64 : 32, NT = CH / 8;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = lane >> 2, q = lane & 3;
-  for (int c0 = lo + CH * warp; c0 < hi; c0 += CH * (kThreads / 32)) {
-    for (int m = 0; m < MT / 16; m++) {
-      if (16 * m >= rows) break;
-      float acc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < RT; ks++) {
-        uint32_t ua[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const uint2 p = *reinterpret_cast<const uint2*>(s_u + (t * MT + 16 * m + i) * UP + 16 * ks + 4 * q);
-          const uint2 v = *reinterpret_cast<const uint2*>(s_u + (t * MT + 16 * m + 8 + i) * UP + 16 * ks + 4 * q);
-          ua[t][0] = p.x; ua[t][1] = v.x; ua[t][2] = p.y; ua[t][3] = v.y;
-        }
-        const int j = 16 * ks + 4 * q;
-        if constexpr (!BWD) {
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            const int col = c0 + 8 * (i >> 1) + 2 * n + (i & 1);
-            Load<PT, 4, VW> w;
-            w.get(w2 + (long long)col * a.r + j, col < hi ? a.r - j : 0);
-            uint32_t b0[PN], b1[PN];
-            pair_along<PT, PN>(w, 0, b0);
-            pair_along<PT, PN>(w, 2, b1);
-            mma_terms<2, PN, 2, CT>(acc[n], ua, b0, b1);
-          }
-        } else {
-          Load<PT, 8, VW> w[4];
-#pragma unroll
-          for (int k = 0; k < 4; k++) w[k].get(w2 + (long long)(j + k) * a.D2 + c0 + 8 * i, j + k < a.r ? hi - (c0 + 8 * i) : 0);
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            uint32_t b0[PN], b1[PN];
-            pair_across<PT, PN>(w[0], w[1], n, b0);
-            pair_across<PT, PN>(w[2], w[3], n, b1);
-            mma_terms<2, PN, 2, CT>(acc[n], ua, b0, b1);
-          }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int row = s_row[16 * m + 8 * h + i];
-        if (row < 0) continue;
-        const float f = s_factor[16 * m + 8 * h + i];
-        float v[8];
-        if constexpr (!BWD) {
-#pragma unroll
-          for (int n = 0; n < 4; n++) { v[2 * n] = acc[n][2 * h]; v[2 * n + 1] = acc[n][2 * h + 1]; }
-          if (c0 + 8 * q < hi) store8<XT>(a, row, c0 + 8 * q, hi, v, f);
-        } else {
-#pragma unroll
-          for (int p = 0; p < 2; p++) {
-#pragma unroll
-            for (int n = 0; n < 8; n++) v[n] = acc[n][2 * h + p];
-            if (c0 + 16 * q + 8 * p < hi) store8<XT>(a, row, c0 + 16 * q + 8 * p, hi, v, f);
-          }
-        }
-      }
-    }
-  }
-}
-
-template <int RT, int MT>
-constexpr int tile_smem() {
-  constexpr int RP = 16 * RT;
-  const int red = kThreads / 32 / 2 * (MT >= 32 ? 32 : 16) * RP * 4;   // the partial sums of half of the warps
-  return red + MT * RP * 4 + 2 * MT * (RP + 8) * 2 + MT * 4 * 2 + 16;
-}
+// ---------------------------------------------------------------------------------------------------- both products
+template <typename PT, bool BWD, int RT, int MT>
+struct Shape {
+  static constexpr int RP = 16 * RT, PS = sizeof(PT), WM = MT / 16, KS = kThreads / 32 / WM;   // KS warps share sixteen rows
+  static constexpr int KB = MT == 64 ? 64 : 128;                 // contraction of a stage of the first product
+  static constexpr int CW = MT == 64 ? 32 : 16, NB = CW * KS;    // columns of a warp and of a stage of the second
+  static constexpr int X = MT * KB * 2, W1 = RP * KB * PS, Y = MT * NB * 2, W2 = NB * RP * PS;
+  static constexpr int STAGE = X + W1 > Y + W2 ? X + W1 : Y + W2;
+  static constexpr int UP = RP + 8;
+  static constexpr int RED = KS / 2 * WM * 16 * RP * 4, PART = MT * RP * 4, U = 2 * MT * UP * 2;
+  static constexpr int REST = RED + PART + U + MT * 8 + 16;
+  static constexpr int FIT = 96 * 1024 / STAGE, STAGES = FIT > 8 ? 8 : FIT >= 3 ? FIT : 3 * STAGE + REST <= 220 * 1024 ? 3 : 2;
+  static constexpr int SMEM = STAGES * STAGE + REST;
+};
 
 template <typename XT, typename PT, bool BWD, int RT, int MT>
 __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
+  typedef Shape<PT, BWD, RT, MT> S;
   typedef typename std::conditional<sizeof(PT) == 4, bf16, XT>::type CT;
-  constexpr int RP = 16 * RT, UP = RP + 8, WT = MT >= 32 ? 2 : 1, TG = MT / (16 * WT), KS = kThreads / 32 / TG;
-  constexpr int JV = 2 * RT;
+  constexpr int RP = S::RP, UP = S::UP, KS = S::KS, WM = S::WM, KB = S::KB, NB = S::NB, CW = S::CW, PS = S::PS;
+  constexpr int XN = RowTerms<XT, CT>::N, P1 = PS == 4 ? 3 : 1, P2 = PS == 4 ? 2 : 1, UT = PS == 4 ? 3 : 2;
+  typedef Tile<KB, 2> XTile;
+  typedef Tile<NB, 2> YTile;
+  constexpr int W1C = BWD ? RP : KB, W2C = BWD ? NB : RP;   // columns of the stages' weight tiles
   extern __shared__ __align__(16) uint8_t smem[];
-  float* s_red = reinterpret_cast<float*>(smem);                                     // [warps / 2][16 WT][RP]
-  float* s_part = s_red + kThreads / 32 / 2 * 16 * WT * RP;                          // [MT][RP]: this CTA's part of u
-  uint16_t* s_u = reinterpret_cast<uint16_t*>(s_part + MT * RP);                     // [2][MT][UP]: u as two terms
-  float* s_factor = reinterpret_cast<float*>(s_u + 2 * MT * UP);                     // [MT]
-  int* s_row = reinterpret_cast<int*>(s_factor + MT);                                // [MT]
+  float* s_red = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE);   // parts of u of half of the warps
+  float* s_part = s_red + S::RED / 4;                                     // [MT][RP]: this CTA's part of u
+  uint16_t* s_u = reinterpret_cast<uint16_t*>(s_part + S::PART / 4);      // [2][MT][UP]: u as two terms
+  float* s_factor = reinterpret_cast<float*>(s_u + S::U / 2);             // [MT]
+  int* s_row = reinterpret_cast<int*>(s_factor + MT);                     // [MT]
   int* s_info = s_row + MT;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, q = lane & 3;
+  const int wm = warp % WM, ks = warp / WM;
   const TileAt t = find_tile<MT>(a, blockIdx.x / C, s_row, s_info);
   if (t.rows == 0) return;   // (the whole cluster)
-  const int chunk = BWD ? 64 : 32, n_chunks = (a.c1 - a.c0 + chunk - 1) / chunk;
-  const int lo = a.c0 + (int)((long long)n_chunks * rank / C) * chunk;
-  const int hi = min(a.c1, a.c0 + (int)((long long)n_chunks * (rank + 1) / C) * chunk);
+  const int n_chunks = (a.c1 - a.c0 + NB - 1) / NB;
+  const int lo = a.c0 + (int)((long long)n_chunks * rank / C) * NB;
+  const int hi = min(a.c1, a.c0 + (int)((long long)n_chunks * (rank + 1) / C) * NB);
   if (t.group < 0) {
     copy_rows<XT>(a, s_row, t.rows, lo, hi);
     if (a.shrink && a.u != nullptr && rank == 0)
-      for (int v = tid; v < t.rows * a.r; v += kThreads) a.u[(long long)s_row[v / a.r] * a.r + v % a.r] = 0.f;
+      for (int v = tid; v < t.rows * UT * a.ru; v += kThreads)
+        a.u[((long long)(v / a.ru % UT) * a.g.n + s_row[v / (a.ru * UT)]) * a.ru + v % a.ru] = 0;
     return;
   }
   const float factor = factor_of(a.g, t.group);
+  const PT* w1 = static_cast<const PT*>(a.w1) + (long long)t.group * a.r * a.D1;
+  const PT* w2 = static_cast<const PT*>(a.w2) + (long long)t.group * a.r * a.D2;
+  const int blocks = a.shrink ? (a.D1 + KB - 1) / KB : 0;
+  const int b0 = (int)((long long)blocks * rank / C), n1 = (int)((long long)blocks * (rank + 1) / C) - b0;
+  const int n2 = a.out != nullptr ? (hi - lo + NB - 1) / NB : 0;
+  const bool staged = a.base != nullptr && a.vec_out;   // the base's rows come with the weights
+  const uint32_t ring = smem_at(smem);
+
+  // Stages 0 .. n1 - 1: rows and weights of the first product; then the second's weights and the base's rows.
+  auto fetch = [&](int s) {
+    const uint32_t at = ring + s % S::STAGES * S::STAGE;
+    if (s < n1) {
+      const int k0 = (b0 + s) * KB;
+#pragma unroll
+      for (int c = tid; c < MT * XTile::CHUNKS; c += kThreads) {
+        const int m = c / XTile::CHUNKS, ch = c % XTile::CHUNKS, e = s_row[m];
+        const XT* row = static_cast<const XT*>(a.in) + (e < 0 ? 0 : (long long)(a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div)) * a.in_stride);
+        load_chunk<2>(XTile::at(at, m, ch), row, k0 + 8 * ch, e < 0 ? 0 : a.D1, a.by_in);
+      }
+      typedef Tile<W1C, PS> W;
+      constexpr int ROWS = BWD ? KB : RP;
+#pragma unroll
+      for (int c = tid; c < ROWS * W::CHUNKS; c += kThreads) {
+        const int m = c / W::CHUNKS, ch = c % W::CHUNKS;
+        if constexpr (BWD) load_chunk<PS>(W::at(at + S::X, m, ch), w1 + (long long)min(k0 + m, a.D1 - 1) * a.r, W::PER * ch, k0 + m < a.D1 ? a.r : 0, a.by_w1);
+        else load_chunk<PS>(W::at(at + S::X, m, ch), w1 + (long long)min(m, a.r - 1) * a.D1, k0 + W::PER * ch, m < a.r ? a.D1 : 0, a.by_w1);
+      }
+    } else if (s < n1 + n2) {
+      const int c0 = lo + (s - n1) * NB;
+      typedef Tile<W2C, PS> W;
+      constexpr int ROWS = BWD ? RP : NB;
+#pragma unroll
+      for (int c = tid; c < ROWS * W::CHUNKS; c += kThreads) {
+        const int m = c / W::CHUNKS, ch = c % W::CHUNKS;
+        if constexpr (BWD) load_chunk<PS>(W::at(at + S::Y, m, ch), w2 + (long long)min(m, a.r - 1) * a.D2, c0 + W::PER * ch, m < a.r ? hi : 0, a.by_w2);
+        else load_chunk<PS>(W::at(at + S::Y, m, ch), w2 + (long long)min(c0 + m, hi - 1) * a.r, W::PER * ch, c0 + m < hi ? a.r : 0, a.by_w2);
+      }
+      if (staged) {
+#pragma unroll
+        for (int c = tid; c < MT * YTile::CHUNKS; c += kThreads) {
+          const int m = c / YTile::CHUNKS, ch = c % YTile::CHUNKS, e = s_row[m];
+          load_chunk<2>(YTile::at(at, m, ch), static_cast<const XT*>(a.base) + (long long)max(e, 0) * a.base_stride, c0 + 8 * ch, e < 0 ? 0 : hi, kBy16);
+        }
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S::STAGES - 1; s++) fetch(s);
+
   if (a.shrink) {
-    const PT* w1 = static_cast<const PT*>(a.w1) + (long long)t.group * a.r * a.D1;
-    const int blocks = (a.D1 + 31) / 32;
-    const int b0 = (int)((long long)blocks * rank / C), b1 = (int)((long long)blocks * (rank + 1) / C);
-    const int tg = warp / KS, ks = warp % KS;
-    float acc[WT][2 * RT][4];
+    float acc[2 * RT][4];
 #pragma unroll
-    for (int m = 0; m < WT; m++)
+    for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-      for (int n = 0; n < 2 * RT; n++)
+      for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+    for (int s = 0; s < n1; s++) {
+      cp_wait<S::STAGES - 2>();
+      __syncthreads();
+      fetch(s + S::STAGES - 1);
+      const uint32_t at = ring + s % S::STAGES * S::STAGE;
+      // The tensor cores cut off what a sum has below its last bit. Where float32 results are wanted, a stage's products are added up
+      // by themselves and then, rounded, to the whole.
+      float part[2 * RT][4];
+      if constexpr (PS == 4) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) acc[m][n][k] = 0.f;
-    if (a.vec_in && a.vec_w1)
-      shrink_part<XT, PT, CT, BWD, RT, WT, true, true>(a, w1, s_row, 16 * WT * tg, 32 * (b0 + ks), 32 * b1, 32 * KS, acc);
-    else
-      shrink_part<XT, PT, CT, BWD, RT, WT, false, false>(a, w1, s_row, 16 * WT * tg, 32 * (b0 + ks), 32 * b1, 32 * KS, acc);
+        for (int n = 0; n < 2 * RT; n++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) part[n][k] = 0.f;
+      }
+#pragma unroll
+      for (int k = ks; k < KB / 16; k += KS) {
+        uint32_t raw[4], xa[XN][4];
+        ldsm(raw, XTile::at(at, 16 * wm + (lane & 15), 2 * k + (lane >> 4)));
+        RowTerms<XT, CT>::get(raw, xa);
+#pragma unroll
+        for (int n = 0; n < RT; n++) {
+          uint32_t b[2][2][P1];
+          load_b<PT, P1, W1C, !BWD>(at + S::X, 16 * n, 16 * k, b);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if constexpr (PS == 4) mma_terms<XN, P1, CT>(part[2 * n + h], xa, b[h][0], b[h][1]);
+            else mma_terms<XN, P1, CT>(acc[2 * n + h], xa, b[h][0], b[h][1]);
+          }
+        }
+      }
+      if constexpr (PS == 4) {
+#pragma unroll
+        for (int n = 0; n < 2 * RT; n++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) acc[n][k] += part[n][k];
+      }
+    }
     // the warps' parts, halves onto halves
+#pragma unroll
     for (int h = KS / 2; h > 0; h >>= 1) {
-      float* mine = s_red + (size_t)(tg * (KS / 2) + (ks % h)) * 16 * WT * RP;
+      float* mine = s_red + (wm * (KS / 2) + ks % h) * 16 * RP;
       if (ks >= h && ks < 2 * h) {
 #pragma unroll
-        for (int m = 0; m < WT; m++)
+        for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-          for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) mine[((m * 2 * RT + n) * 4 + k) * 32 + lane] = acc[m][n][k];
+          for (int k = 0; k < 4; k++) mine[(n * 4 + k) * 32 + lane] = acc[n][k];
       }
       __syncthreads();
       if (ks < h) {
 #pragma unroll
-        for (int m = 0; m < WT; m++)
+        for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-          for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) acc[m][n][k] += mine[((m * 2 * RT + n) * 4 + k) * 32 + lane];
+          for (int k = 0; k < 4; k++) acc[n][k] += mine[(n * 4 + k) * 32 + lane];
       }
       __syncthreads();
     }
     if (ks == 0) {
 #pragma unroll
-      for (int m = 0; m < WT; m++)
+      for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-        for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const int row = 16 * (WT * tg + m) + i + 8 * (k >> 1), c = 2 * q + (k & 1);
-            s_part[row * RP + (BWD ? c * JV + n : 8 * n + c)] = acc[m][n][k];
-          }
+        for (int k = 0; k < 4; k++) s_part[(16 * wm + i + 8 * (k >> 1)) * RP + 8 * n + 2 * q + (k & 1)] = acc[n][k];
     }
     cluster.sync();
   }
-  // u of the whole contraction: float32 out, two terms for the second product. A warp a row at a time.
+  // u of the whole contraction, saved as bf16 terms and as two terms for the second product. A warp a row at a time.
   for (int m = warp; m < MT; m += kThreads / 32) {
     float v[(RP + 31) / 32], most = 0.f;
     const int row = s_row[m];
@@ -507,10 +460,16 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
         if (a.shrink) {
           for (int c = 0; c < C; c++) v[b] += *cluster.map_shared_rank(s_part + m * RP + j, c);
           if (a.scale_u) v[b] *= factor;
-          if (a.u != nullptr && rank == m % C) a.u[(long long)row * a.r + j] = v[b];
         } else {
-          v[b] = a.u[(long long)row * a.r + j];
+#pragma unroll
+          for (int n = UT - 1; n >= 0; n--) v[b] += __uint_as_float((uint32_t)a.u[((long long)n * a.g.n + row) * a.ru + j] << 16);
         }
+      }
+      if (j < a.ru && row >= 0 && a.shrink && a.u != nullptr && rank == m % C) {
+        uint32_t p[UT];
+        split<UT>(v[b], 0.f, p);
+#pragma unroll
+        for (int n = 0; n < UT; n++) a.u[((long long)n * a.g.n + row) * a.ru + j] = (uint16_t)p[n];
       }
       most = fmaxf(most, fabsf(v[b]));
     }
@@ -532,28 +491,101 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
         s_u[m * UP + j] = __half_as_ushort(h);
         s_u[(MT + m) * UP + j] = __half_as_ushort(__float2half_rn(rest));
       } else {
-        const uint32_t h = __float_as_uint(v[b]) & 0xffff0000u;
-        const float rest = fabsf(v[b]) == INFINITY ? 0.f : v[b] - __uint_as_float(h);
-        s_u[m * UP + j] = (uint16_t)(h >> 16);
-        s_u[(MT + m) * UP + j] = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
+        uint32_t p[2];
+        split<2>(v[b], 0.f, p);
+        s_u[m * UP + j] = (uint16_t)p[0];
+        s_u[(MT + m) * UP + j] = (uint16_t)p[1];
       }
     }
     if (lane == 0) s_factor[m] = a.scale_u ? f : f * factor;
   }
   __syncthreads();
   if (a.shrink) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-  if (a.out != nullptr) {
-    const PT* w2 = static_cast<const PT*>(a.w2) + (long long)t.group * a.r * a.D2;
-    if (a.vec_w2) expand_part<XT, PT, CT, BWD, RT, MT, true>(a, w2, s_row, s_factor, s_u, t.rows, lo, hi);
-    else expand_part<XT, PT, CT, BWD, RT, MT, false>(a, w2, s_row, s_factor, s_u, t.rows, lo, hi);
+
+  const uint32_t u_at = smem_at(s_u);
+  for (int s = n1; s < n1 + n2; s++) {
+    cp_wait<S::STAGES - 2>();
+    __syncthreads();
+    fetch(s + S::STAGES - 1);
+    const uint32_t at = ring + s % S::STAGES * S::STAGE;
+    const int c0 = lo + (s - n1) * NB, cw = CW * ks;
+    if (16 * wm >= t.rows || c0 + cw >= hi) continue;
+    float acc[CW / 8][4];
+#pragma unroll
+    for (int n = 0; n < CW / 8; n++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+#pragma unroll
+    for (int k = 0; k < RT; k++) {
+      uint32_t ua[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; n++) ldsm(ua[n], u_at + ((n * MT + 16 * wm + (lane & 15)) * UP + 16 * k + 8 * (lane >> 4)) * 2);
+#pragma unroll
+      for (int n = 0; n < CW / 16; n++) {
+        uint32_t b[2][2][P2];
+        load_b<PT, P2, W2C, !BWD>(at + S::Y, cw + 16 * n, 16 * k, b);
+#pragma unroll
+        for (int h = 0; h < 2; h++) mma_terms<2, P2, CT>(acc[2 * n + h], ua, b[h][0], b[h][1]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int m = 16 * wm + 8 * h + i, row = s_row[m];
+      const float f = s_factor[m];
+      if (a.vec_out && !a.out_f32) {
+        // in the stage's room for the base's rows, from where whole chunks leave
+#pragma unroll
+        for (int n = 0; n < CW / 8; n++) {
+          const uint32_t p = YTile::at(at, m, cw / 8 + n) + 4 * q;
+          float y0 = 0.f, y1 = 0.f;
+          if (staged) {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(p) : "memory");
+            const XT* y = reinterpret_cast<const XT*>(&v);
+            y0 = to_float(y[0]);
+            y1 = to_float(y[1]);
+          }
+          XT o[2] = {XT(fmaf(f, acc[n][2 * h], y0)), XT(fmaf(f, acc[n][2 * h + 1], y1))};
+          asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(p), "r"(*reinterpret_cast<const uint32_t*>(o)) : "memory");
+        }
+      } else if (row >= 0) {
+#pragma unroll
+        for (int n = 0; n < CW / 8; n++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const int col = c0 + cw + 8 * n + 2 * q + k;
+            if (col >= hi) continue;
+            if (a.out_f32) {
+              static_cast<float*>(a.out)[(long long)row * a.out_stride + col - a.c0] = f * acc[n][2 * h + k];
+            } else {
+              const float y = a.base != nullptr ? to_float(static_cast<const XT*>(a.base)[(long long)row * a.base_stride + col]) : 0.f;
+              static_cast<XT*>(a.out)[(long long)row * a.out_stride + col] = XT(fmaf(f, acc[n][2 * h + k], y));
+            }
+          }
+      }
+    }
+    if (a.vec_out && !a.out_f32) {
+      __syncwarp();
+      constexpr int EACH = CW / 8;   // chunks of a row
+#pragma unroll
+      for (int c = lane; c < 16 * EACH; c += 32) {
+        const int m = 16 * wm + c / EACH, ch = cw / 8 + c % EACH, row = s_row[m], col = c0 + 8 * ch;
+        if (row < 0 || col >= hi) continue;
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(YTile::at(at, m, ch)) : "memory");
+        *reinterpret_cast<uint4*>(static_cast<XT*>(a.out) + (long long)row * a.out_stride + col) = v;
+      }
+    }
   }
+  cp_wait<0>();
   // nobody leaves while its part of u may still be read
+  __syncthreads();
   if (a.shrink) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
 template <typename XT, typename PT, bool BWD, int RT, int MT>
 cudaError_t launch_tile(const LoraArgs& a, int cluster, cudaStream_t st) {
-  constexpr int smem = tile_smem<RT, MT>();
+  constexpr int smem = Shape<PT, BWD, RT, MT>::SMEM;
   auto kern = tile_kernel<XT, PT, BWD, RT, MT>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

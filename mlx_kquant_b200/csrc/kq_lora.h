@@ -54,13 +54,15 @@ struct LoraArgs {
   long long out_stride;
   int out_f32;                // out is float32 and base nullptr
   int c0, c1;                 // columns [c0, c1) of out; column c is stored at c - c0
-  float* u;                   // [n, r]: written by the shrink (if not nullptr), read where shrink == 0
+  uint16_t* u;                // [terms][n][ru] bf16 terms: written by the shrink (if not nullptr), read where shrink == 0
+  int ru;                     // r up to a multiple of 8
   int shrink;
   int scale_u;                // the factor goes into u (backward), not into the output
   LoraPlan plan;              // tiles == nullptr: one group, rows in order; or `direct`
   int direct;                 // tiles are found by the kernel itself: cluster c looks for the tile that entry c leads
   int n_clusters;             // tiles
-  int vec_in, vec_w1, vec_w2, vec_out;  // rows are whole groups of elements that start aligned
+  int by_in, by_w1, by_w2;    // how rows are read: by 16 bytes, 8, or elements
+  int vec_out;                // rows of base and out are whole aligned groups of 16 bytes
 };
 enum LoraTypes { kLoraBf16 = 0, kLoraF16 = 1, kLoraBf16F32 = 2, kLoraF16F32 = 3 };  // rows, and parameters where they are float32
 cudaError_t launch_lora_tile_bf16(const LoraArgs& a, bool backward, int mt, int cluster, cudaStream_t st);
@@ -74,14 +76,14 @@ struct LoraWgradArgs {
   const void* in;
   long long in_stride;
   int in_div, D, r;
-  const float* uv;       // [n, r]
+  const uint16_t* uv;    // [terms][n][ru]
+  int ru;
   int scaled;            // times the adapter's factor
   void* out;
   int r_first;           // out [groups, r, D], else [groups, D, r]
   const int *order, *offsets;  // or nullptr: one group, rows in order
   int n_groups;
-  int splits;            // warps of a CTA that share a column tile: 1, 2, 4, 8
-  int vec_in;
+  int by_in;
 };
 cudaError_t launch_lora_wgrad(const LoraWgradArgs& a, int in_dtype, int out_f32, int cluster, cudaStream_t st);
 
@@ -99,10 +101,11 @@ struct LoraCall {
   const void *a, *b;
   const void* plan;          // or nullptr
 };
-cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_stride, void* out, long long out_stride, float* u,
+cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_stride, void* out, long long out_stride, void* u,
                                 cudaStream_t st);
-size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int r);
-cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy_stride, const float* u, void* dx, long long dx_stride,
+size_t lora_saved_bytes(long long n, int r, int param_f32);
+size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int r, int param_f32);
+cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy_stride, const void* u, void* dx, long long dx_stride,
                                  void* da, void* db, void* workspace, cudaStream_t st);
 
 }  // namespace kq

@@ -81,7 +81,7 @@ class _Call:
         da = torch.empty_like(a) if need_a else None
         db = torch.empty_like(b) if need_b else None
         L = _lib.lib()
-        ws = torch.empty(max(256, L.kq_lora_backward_workspace_bytes(rows, self.slots, int(self.shared), K, r)),
+        ws = torch.empty(max(256, L.kq_lora_backward_workspace_bytes(rows, self.slots, int(self.shared), K, r, _DT[a.dtype])),
                          dtype=torch.uint8, device=dev)
         with _on_device(dev):
             check(L.kq_lora_backward(
@@ -97,7 +97,7 @@ class _Update(torch.autograd.Function):
     def forward(ctx, call, y, x, a, b):
         rows = y.numel() // y.shape[-1]
         plan = call.plan(rows, x.device)
-        u = torch.empty((rows, a.shape[-2]), dtype=torch.float32, device=x.device)
+        u = torch.empty(_lib.lib().kq_lora_saved_bytes(rows, a.shape[-2], _DT[a.dtype]), dtype=torch.uint8, device=x.device)
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
         call.forward(y, x, a, b, out, u, plan)
         ctx.call = call
