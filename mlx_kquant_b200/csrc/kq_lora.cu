@@ -110,9 +110,10 @@ struct WgradShape {
   static constexpr int IN = ROWS * COLS * 2, UV = ROWS * RP * 2, STAGE = IN + UN * UV;
   static constexpr int STAGES = 96 * 1024 / STAGE > 5 ? 5 : 96 * 1024 / STAGE < 3 ? 3 : 96 * 1024 / STAGE;
   static constexpr int OUT = COLS * RP * 4;   // sums of a half of the warps, then of the CTA: in the ring's room
-  static constexpr int SMEM = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+  static constexpr int RING = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+  static constexpr int SMEM = RING + (STAGES + 1) * ROWS * 4;   // and the entries of the stages
 };
-template <typename XT, typename PT, int RT>
+template <typename XT, typename PT, int RT, bool FAST>
 __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) {
   typedef WgradShape<PT, RT> S;
   constexpr int XN = RowTerms<XT, bf16>::N, UN = S::UN, RP = S::RP;
@@ -131,28 +132,50 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
   const int blocks = (count + S::ROWS - 1) / S::ROWS;
   const int b0 = (int)((long long)blocks * rank / C), nb = (int)((long long)blocks * (rank + 1) / C) - b0;
   const uint32_t ring = smem_at(smem);
-  auto fetch = [&](int s) {
-    if (s < nb) {
-      const uint32_t at = ring + s % S::STAGES * S::STAGE;
-      const int t0 = (b0 + s) * S::ROWS;
+  // Entries of the stages, known a stage before their rows are asked for: read two stages ahead into a register, then put here.
+  int* s_entry = reinterpret_cast<int*>(smem + S::RING);
+  auto entry_of = [&](int s) {
+    const int t = (b0 + s) * S::ROWS + tid;
+    return tid >= S::ROWS || s >= nb || t >= count ? -1 : a.order != nullptr ? a.order[start + t] : t;
+  };
+  typedef Deal<S::ROWS, S::COLS, 2> InD;
+  const uint32_t in_to = InTile::at(0, InD::row(), InD::chunk());
+  const int col = c0 + 8 * InD::chunk();
+  int next = 0, into = 0, listed = 0;
+  int upcoming = entry_of(S::STAGES);
+  auto fetch = [&]() {
+    const uint32_t at = ring + into * S::STAGE;
+    into = into + 1 == S::STAGES ? 0 : into + 1;
+    if (next < nb) {
+      const int* entries = s_entry + listed * S::ROWS;
 #pragma unroll
-      for (int c = tid; c < S::ROWS * InTile::CHUNKS; c += kThreads) {
-        const int m = c / InTile::CHUNKS, ch = c % InTile::CHUNKS, t = t0 + m;
-        int e = t >= count ? -1 : a.order != nullptr ? a.order[start + t] : t;
-        const int row = e < 0 ? 0 : a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div);
-        load_chunk<2>(InTile::at(at, m, ch), static_cast<const XT*>(a.in) + (long long)row * a.in_stride, c0 + 8 * ch, e < 0 ? 0 : a.D, a.by_in);
+      for (int k = 0; k < InD::EACH; k++) {
+        const int e = entries[InD::row() + k * InD::STEP];
+        const int row = e < 0 || a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div);
+        const XT* p = static_cast<const XT*>(a.in) + (long long)row * a.in_stride;
+        const uint32_t to = at + in_to + k * InD::STEP * InTile::CHUNKS * 16;
+        if constexpr (FAST) cp16(to, e >= 0 && col < a.D ? p + col : a.in, e >= 0 && col < a.D);
+        else load_chunk<2>(to, e >= 0 ? p : a.in, col, e >= 0 ? a.D : 0, a.by_in);
       }
 #pragma unroll
-      for (int c = tid; c < UN * S::ROWS * UvTile::CHUNKS; c += kThreads) {
-        const int n = c / (S::ROWS * UvTile::CHUNKS), m = c / UvTile::CHUNKS % S::ROWS, ch = c % UvTile::CHUNKS, t = t0 + m;
-        const int e = t >= count ? -1 : a.order != nullptr ? a.order[start + t] : t;
-        load_chunk<2>(UvTile::at(at + S::IN + n * S::UV, m, ch), a.uv + ((long long)n * a.g.n + max(e, 0)) * a.ru, j0 + 8 * ch, e < 0 ? 0 : a.ru, kBy16);
-      }
+      for (int n = 0; n < UN; n++)
+#pragma unroll
+        for (int c = tid; c < S::ROWS * UvTile::CHUNKS; c += kThreads) {
+          const int m = c / UvTile::CHUNKS, ch = c % UvTile::CHUNKS, e = entries[m];
+          const bool there = e >= 0 && j0 + 8 * ch < a.ru;
+          cp16(UvTile::at(at + S::IN + n * S::UV, m, ch), there ? a.uv + ((long long)n * a.g.n + e) * a.ru + j0 + 8 * ch : a.uv, there);
+        }
     }
+    next++;
+    listed = listed == S::STAGES ? 0 : listed + 1;
     cp_commit();
   };
-#pragma unroll
-  for (int s = 0; s < S::STAGES - 1; s++) fetch(s);
+  for (int s = 0; s < S::STAGES; s++)
+    if (tid < S::ROWS) s_entry[s * S::ROWS + tid] = entry_of(s);
+  __syncthreads();
+#pragma unroll 1
+  for (int s = 0; s < S::STAGES - 1; s++) fetch();
+  int put = S::STAGES;   // where the entries of stage s + STAGES go
   float acc[2][2 * RT][4];
 #pragma unroll
   for (int m = 0; m < 2; m++)
@@ -163,7 +186,11 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
   for (int s = 0; s < nb; s++) {
     cp_wait<S::STAGES - 2>();
     __syncthreads();
-    fetch(s + S::STAGES - 1);
+    fetch();
+    // (the slot's last reader, the fetch of stage s - 1, lies behind the barrier)
+    if (tid < S::ROWS) s_entry[put * S::ROWS + tid] = upcoming;
+    put = put == S::STAGES ? 0 : put + 1;
+    upcoming = entry_of(s + S::STAGES + 1);
     const uint32_t at = ring + s % S::STAGES * S::STAGE;
     const int left = count - (b0 + s) * S::ROWS;
     float part[2][2 * RT][4];   // (a stage's sums by themselves: see the tile kernel)
@@ -247,10 +274,10 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
   if (C > 1) cluster.sync();
 }
 
-template <typename XT, typename PT, int RT>
+template <typename XT, typename PT, int RT, bool FAST>
 cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
   typedef WgradShape<PT, RT> S;
-  auto kern = wgrad_kernel<XT, PT, RT>;
+  auto kern = wgrad_kernel<XT, PT, RT, FAST>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -265,11 +292,15 @@ cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
-template <typename XT, typename PT>
+template <typename XT, typename PT, bool FAST>
 cudaError_t wgrad_rank(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
-  if (a.r <= 16) return wgrad_launch<XT, PT, 1>(a, cluster, st);
-  if (a.r <= 32) return wgrad_launch<XT, PT, 2>(a, cluster, st);
-  return wgrad_launch<XT, PT, 4>(a, cluster, st);
+  if (a.r <= 16) return wgrad_launch<XT, PT, 1, FAST>(a, cluster, st);
+  if (a.r <= 32) return wgrad_launch<XT, PT, 2, FAST>(a, cluster, st);
+  return wgrad_launch<XT, PT, 4, FAST>(a, cluster, st);
+}
+template <typename XT, typename PT>
+cudaError_t wgrad_read(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
+  return a.by_in == kBy16 ? wgrad_rank<XT, PT, true>(a, cluster, st) : wgrad_rank<XT, PT, false>(a, cluster, st);
 }
 
 // ---------------------------------------------------------------------------------------------------- sum over slots
@@ -377,8 +408,8 @@ cudaError_t launch_lora_plan(const LoraGroups& g, void* plan, cudaStream_t st) {
 }
 
 cudaError_t launch_lora_wgrad(const LoraWgradArgs& a, int in_dtype, int out_f32, int cluster, cudaStream_t st) {
-  if (in_dtype == 1) return out_f32 ? wgrad_rank<__half, float>(a, cluster, st) : wgrad_rank<__half, __half>(a, cluster, st);
-  return out_f32 ? wgrad_rank<bf16, float>(a, cluster, st) : wgrad_rank<bf16, bf16>(a, cluster, st);
+  if (in_dtype == 1) return out_f32 ? wgrad_read<__half, float>(a, cluster, st) : wgrad_read<__half, __half>(a, cluster, st);
+  return out_f32 ? wgrad_read<bf16, float>(a, cluster, st) : wgrad_read<bf16, bf16>(a, cluster, st);
 }
 
 cudaError_t launch_lora_sum_slots(const float* part, int slots, long long tokens, int cols, void* out, long long out_stride, int dtype,

@@ -132,6 +132,9 @@ struct Tile {
   __device__ static __forceinline__ uint32_t at(uint32_t base, int row, int c) { return base + 16 * chunk(row, c); }
 };
 
+template <int ES>
+__device__ __forceinline__ constexpr int PerChunk() { return 16 / ES; }
+
 // how a matrix's rows can be read: 16 bytes at a time, 8, or element by element
 enum { kBy16 = 0, kBy8 = 1, kByElement = 2 };
 
@@ -289,25 +292,54 @@ struct Shape {
   static constexpr int X = MT * KB * 2, W1 = RP * KB * PS, Y = MT * NB * 2, W2 = NB * RP * PS;
   static constexpr int STAGE = X + W1 > Y + W2 ? X + W1 : Y + W2;
   static constexpr int UP = RP + 8;
-  static constexpr int RED = KS / 2 * WM * 16 * RP * 4, PART = MT * RP * 4, U = 2 * MT * UP * 2;
-  static constexpr int REST = RED + PART + U + MT * 8 + 16;
-  static constexpr int FIT = 96 * 1024 / STAGE, STAGES = FIT > 8 ? 8 : FIT >= 3 ? FIT : 3 * STAGE + REST <= 220 * 1024 ? 3 : 2;
+  // the sums of half of the warps, and then the CTA's part of u, in one place
+  static constexpr int RED = KS / 2 * WM * 16 * RP * 4, PART = MT * RP * 4, SUM = RED > PART ? RED : PART, U = 2 * MT * UP * 2;
+  static constexpr int REST = SUM + U + MT * 8 + 16;
+  // two CTAs of an SM where at least four stages of each fit, else one
+  static constexpr int TWO = (112 * 1024 - REST) / STAGE, ONE = (224 * 1024 - REST) / STAGE;
+  static constexpr int STAGES = TWO >= 4 ? (TWO > 8 ? 8 : TWO) : ONE > 6 ? 6 : ONE;
   static constexpr int SMEM = STAGES * STAGE + REST;
+  static_assert(STAGES >= 2 && SMEM <= 227 * 1024, "does not fit");
 };
 
-template <typename XT, typename PT, bool BWD, int RT, int MT>
+// One matrix of a stage: ROWS x COLS elements, chunks dealt out to the threads; with a thread's chunks a fixed number of rows apart.
+template <int ROWS, int COLS, int ES>
+struct Deal {
+  typedef Tile<COLS, ES> T;
+  static constexpr int CHUNKS = ROWS * T::CHUNKS, EACH = (CHUNKS + kThreads - 1) / kThreads, STEP = kThreads / T::CHUNKS;
+  static constexpr bool ALL = CHUNKS % kThreads == 0;   // every thread has EACH chunks
+  static_assert(STEP % 8 == 0, "the permutation of a row's chunks would change");
+  __device__ static __forceinline__ int row() { return threadIdx.x / T::CHUNKS; }
+  __device__ static __forceinline__ int chunk() { return threadIdx.x % T::CHUNKS; }
+  __device__ static __forceinline__ bool has(int t) { return ALL || (int)threadIdx.x + t * kThreads < CHUNKS; }
+};
+
+// Forward, the second product's columns: a warp's tile of CW columns lies in shared memory so that a lane comes to hold CW / 4
+// neighbouring columns of a row of the output. Column n of the stage goes to this row.
+template <int CW>
+__device__ __forceinline__ int place_of(int n) {
+  if constexpr (CW == 32) return (n & ~31) | (n >> 1 & 3) << 3 | (n >> 3 & 3) << 1 | (n & 1);
+  else return (n & ~15) | (n >> 1 & 1) << 3 | (n >> 2 & 3) << 1 | (n & 1);
+}
+
+// FAST: all rows are whole aligned groups of 16 bytes.
+template <typename XT, typename PT, bool BWD, int RT, int MT, bool FAST>
 __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
   typedef Shape<PT, BWD, RT, MT> S;
   typedef typename std::conditional<sizeof(PT) == 4, bf16, XT>::type CT;
   constexpr int RP = S::RP, UP = S::UP, KS = S::KS, WM = S::WM, KB = S::KB, NB = S::NB, CW = S::CW, PS = S::PS;
   constexpr int XN = RowTerms<XT, CT>::N, P1 = PS == 4 ? 3 : 1, P2 = PS == 4 ? 2 : 1, UT = PS == 4 ? 3 : 2;
-  typedef Tile<KB, 2> XTile;
-  typedef Tile<NB, 2> YTile;
   constexpr int W1C = BWD ? RP : KB, W2C = BWD ? NB : RP;   // columns of the stages' weight tiles
+  typedef Deal<MT, KB, 2> XD;
+  typedef Deal<BWD ? KB : RP, W1C, PS> W1D;
+  typedef Deal<BWD ? RP : NB, W2C, PS> W2D;
+  typedef Deal<MT, NB, 2> YD;
+  typedef typename XD::T XTile;
+  typedef typename YD::T YTile;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* s_red = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE);   // parts of u of half of the warps
-  float* s_part = s_red + S::RED / 4;                                     // [MT][RP]: this CTA's part of u
-  uint16_t* s_u = reinterpret_cast<uint16_t*>(s_part + S::PART / 4);      // [2][MT][UP]: u as two terms
+  float* s_red = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE);   // sums of half of the warps
+  float* s_part = s_red;                                                  // then [MT][RP]: this CTA's part of u
+  uint16_t* s_u = reinterpret_cast<uint16_t*>(s_red + S::SUM / 4);        // [2][MT][UP]: u as two terms
   float* s_factor = reinterpret_cast<float*>(s_u + S::U / 2);             // [MT]
   int* s_row = reinterpret_cast<int*>(s_factor + MT);                     // [MT]
   int* s_info = s_row + MT;
@@ -318,8 +350,8 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
   const TileAt t = find_tile<MT>(a, blockIdx.x / C, s_row, s_info);
   if (t.rows == 0) return;   // (the whole cluster)
   const int n_chunks = (a.c1 - a.c0 + NB - 1) / NB;
-  const int lo = a.c0 + (int)((long long)n_chunks * rank / C) * NB;
-  const int hi = min(a.c1, a.c0 + (int)((long long)n_chunks * (rank + 1) / C) * NB);
+  const int lo = a.c0 + n_chunks * rank / C * NB;
+  const int hi = min(a.c1, a.c0 + n_chunks * (rank + 1) / C * NB);
   if (t.group < 0) {
     copy_rows<XT>(a, s_row, t.rows, lo, hi);
     if (a.shrink && a.u != nullptr && rank == 0)
@@ -331,52 +363,79 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
   const PT* w1 = static_cast<const PT*>(a.w1) + (long long)t.group * a.r * a.D1;
   const PT* w2 = static_cast<const PT*>(a.w2) + (long long)t.group * a.r * a.D2;
   const int blocks = a.shrink ? (a.D1 + KB - 1) / KB : 0;
-  const int b0 = (int)((long long)blocks * rank / C), n1 = (int)((long long)blocks * (rank + 1) / C) - b0;
+  const int b0 = blocks * rank / C, n1 = blocks * (rank + 1) / C - b0;
   const int n2 = a.out != nullptr ? (hi - lo + NB - 1) / NB : 0;
   const bool staged = a.base != nullptr && a.vec_out;   // the base's rows come with the weights
   const uint32_t ring = smem_at(smem);
 
-  // Stages 0 .. n1 - 1: rows and weights of the first product; then the second's weights and the base's rows.
-  auto fetch = [&](int s) {
-    const uint32_t at = ring + s % S::STAGES * S::STAGE;
-    if (s < n1) {
-      const int k0 = (b0 + s) * KB;
+  // this thread's chunks: where they come from in the first stage of each product, and where they go
+  const XT *xp[XD::EACH], *yp[YD::EACH];
 #pragma unroll
-      for (int c = tid; c < MT * XTile::CHUNKS; c += kThreads) {
-        const int m = c / XTile::CHUNKS, ch = c % XTile::CHUNKS, e = s_row[m];
-        const XT* row = static_cast<const XT*>(a.in) + (e < 0 ? 0 : (long long)(a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div)) * a.in_stride);
-        load_chunk<2>(XTile::at(at, m, ch), row, k0 + 8 * ch, e < 0 ? 0 : a.D1, a.by_in);
+  for (int k = 0; k < XD::EACH; k++) {
+    const int e = s_row[XD::row() + k * XD::STEP];
+    xp[k] = e < 0 ? nullptr : static_cast<const XT*>(a.in) + (long long)(a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div)) * a.in_stride + b0 * KB;
+  }
+#pragma unroll
+  for (int k = 0; k < YD::EACH; k++) {
+    const int e = YD::has(k) ? s_row[YD::row() + k * YD::STEP] : -1;
+    yp[k] = e < 0 || !staged ? nullptr : static_cast<const XT*>(a.base) + (long long)e * a.base_stride + lo;
+  }
+  const uint32_t x_to = XTile::at(0, XD::row(), XD::chunk()), w1_to = S::X + W1D::T::at(0, W1D::row(), W1D::chunk());
+  const uint32_t y_to = YTile::at(0, YD::row(), YD::chunk());
+  // rows of the first weight matrix: the ranks (forward), or the contraction
+  const long long l1 = BWD ? a.r : a.D1, l2 = BWD ? a.D2 : a.r;
+  const PT* p1 = w1 + (BWD ? (long long)b0 * KB * l1 : (long long)b0 * KB);
+  const PT* p2 = w2 + (BWD ? (long long)lo : (long long)lo * l2);
+
+  int next = 0, into = 0;   // the stage to be fetched, its place in the ring
+  auto fetch = [&]() {
+    const uint32_t at = ring + into * S::STAGE;
+    into = into + 1 == S::STAGES ? 0 : into + 1;
+    if (next < n1) {
+      const int k0 = next * KB, left = a.D1 - b0 * KB - k0;   // of the contraction
+#pragma unroll
+      for (int k = 0; k < XD::EACH; k++) {
+        const int c = PerChunk<2>() * XD::chunk();
+        if constexpr (FAST) cp16(at + x_to + k * XD::STEP * XTile::CHUNKS * 16, xp[k] != nullptr && c < left ? xp[k] + k0 + c : static_cast<const XT*>(a.in), xp[k] != nullptr && c < left);
+        else load_chunk<2>(at + x_to + k * XD::STEP * XTile::CHUNKS * 16, xp[k] != nullptr ? xp[k] + k0 : a.in, c, xp[k] != nullptr ? left : 0, a.by_in);
       }
-      typedef Tile<W1C, PS> W;
-      constexpr int ROWS = BWD ? KB : RP;
 #pragma unroll
-      for (int c = tid; c < ROWS * W::CHUNKS; c += kThreads) {
-        const int m = c / W::CHUNKS, ch = c % W::CHUNKS;
-        if constexpr (BWD) load_chunk<PS>(W::at(at + S::X, m, ch), w1 + (long long)min(k0 + m, a.D1 - 1) * a.r, W::PER * ch, k0 + m < a.D1 ? a.r : 0, a.by_w1);
-        else load_chunk<PS>(W::at(at + S::X, m, ch), w1 + (long long)min(m, a.r - 1) * a.D1, k0 + W::PER * ch, m < a.r ? a.D1 : 0, a.by_w1);
+      for (int k = 0; k < W1D::EACH; k++) {
+        if (!W1D::has(k)) continue;
+        const int m = W1D::row() + k * W1D::STEP, c = PerChunk<PS>() * W1D::chunk();
+        const uint32_t to = at + w1_to + k * W1D::STEP * W1D::T::CHUNKS * 16;
+        const PT* row = p1 + m * l1 + (BWD ? (long long)k0 * l1 : (long long)k0);
+        const bool there = BWD ? m < left : m < a.r;
+        const int most = BWD ? a.r : left;
+        if constexpr (FAST) cp16(to, there && c < most ? row + c : w1, there && c < most);
+        else load_chunk<PS>(to, there ? row : w1, c, there ? most : 0, a.by_w1);
       }
-    } else if (s < n1 + n2) {
-      const int c0 = lo + (s - n1) * NB;
-      typedef Tile<W2C, PS> W;
-      constexpr int ROWS = BWD ? RP : NB;
+    } else if (next < n1 + n2) {
+      const int c0 = (next - n1) * NB, left = hi - lo - c0;   // of the columns
 #pragma unroll
-      for (int c = tid; c < ROWS * W::CHUNKS; c += kThreads) {
-        const int m = c / W::CHUNKS, ch = c % W::CHUNKS;
-        if constexpr (BWD) load_chunk<PS>(W::at(at + S::Y, m, ch), w2 + (long long)min(m, a.r - 1) * a.D2, c0 + W::PER * ch, m < a.r ? hi : 0, a.by_w2);
-        else load_chunk<PS>(W::at(at + S::Y, m, ch), w2 + (long long)min(c0 + m, hi - 1) * a.r, W::PER * ch, c0 + m < hi ? a.r : 0, a.by_w2);
+      for (int k = 0; k < W2D::EACH; k++) {
+        if (!W2D::has(k)) continue;
+        const int m = W2D::row() + k * W2D::STEP, c = PerChunk<PS>() * W2D::chunk();
+        const uint32_t to = at + S::Y + W2D::T::at(0, BWD ? m : place_of<CW>(m), W2D::chunk());
+        const PT* row = p2 + m * l2 + (BWD ? (long long)c0 : (long long)c0 * l2);
+        const bool there = BWD ? m < a.r : m < left;
+        const int most = BWD ? left : a.r;
+        if constexpr (FAST) cp16(to, there && c < most ? row + c : w2, there && c < most);
+        else load_chunk<PS>(to, there ? row : w2, c, there ? most : 0, a.by_w2);
       }
-      if (staged) {
 #pragma unroll
-        for (int c = tid; c < MT * YTile::CHUNKS; c += kThreads) {
-          const int m = c / YTile::CHUNKS, ch = c % YTile::CHUNKS, e = s_row[m];
-          load_chunk<2>(YTile::at(at, m, ch), static_cast<const XT*>(a.base) + (long long)max(e, 0) * a.base_stride, c0 + 8 * ch, e < 0 ? 0 : hi, kBy16);
-        }
+      for (int k = 0; k < YD::EACH; k++) {
+        const int c = PerChunk<2>() * YD::chunk();
+        if (yp[k] != nullptr) cp16(at + y_to + k * YD::STEP * YTile::CHUNKS * 16, c < left ? yp[k] + c0 + c : yp[k], c < left);
       }
     }
+    next++;
     cp_commit();
   };
-#pragma unroll
-  for (int s = 0; s < S::STAGES - 1; s++) fetch(s);
+#pragma unroll 1
+  for (int s = 0; s < S::STAGES - 1; s++) fetch();
+  uint32_t at = ring;   // the stage that is next to be multiplied
+  auto advance = [&]() { at = at + S::STAGE == ring + S::STAGES * S::STAGE ? ring : at + S::STAGE; };
 
   if (a.shrink) {
     float acc[2 * RT][4];
@@ -384,11 +443,11 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
     for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
       for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+#pragma unroll 1
     for (int s = 0; s < n1; s++) {
       cp_wait<S::STAGES - 2>();
       __syncthreads();
-      fetch(s + S::STAGES - 1);
-      const uint32_t at = ring + s % S::STAGES * S::STAGE;
+      fetch();
       // The tensor cores cut off what a sum has below its last bit. Where float32 results are wanted, a stage's products are added up
       // by themselves and then, rounded, to the whole.
       float part[2 * RT][4];
@@ -399,14 +458,15 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
           for (int k = 0; k < 4; k++) part[n][k] = 0.f;
       }
 #pragma unroll
-      for (int k = ks; k < KB / 16; k += KS) {
+      for (int k = 0; k < KB / 16 / KS; k++) {
+        const int step = ks + k * KS;
         uint32_t raw[4], xa[XN][4];
-        ldsm(raw, XTile::at(at, 16 * wm + (lane & 15), 2 * k + (lane >> 4)));
+        ldsm(raw, XTile::at(at, 16 * wm + (lane & 15), 2 * step + (lane >> 4)));
         RowTerms<XT, CT>::get(raw, xa);
 #pragma unroll
         for (int n = 0; n < RT; n++) {
           uint32_t b[2][2][P1];
-          load_b<PT, P1, W1C, !BWD>(at + S::X, 16 * n, 16 * k, b);
+          load_b<PT, P1, W1C, !BWD>(at + S::X, 16 * n, 16 * step, b);
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             if constexpr (PS == 4) mma_terms<XN, P1, CT>(part[2 * n + h], xa, b[h][0], b[h][1]);
@@ -420,6 +480,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
 #pragma unroll
           for (int k = 0; k < 4; k++) acc[n][k] += part[n][k];
       }
+      advance();
     }
     // the warps' parts, halves onto halves
 #pragma unroll
@@ -427,16 +488,18 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
       float* mine = s_red + (wm * (KS / 2) + ks % h) * 16 * RP;
       if (ks >= h && ks < 2 * h) {
 #pragma unroll
-        for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) mine[(n * 4 + k) * 32 + lane] = acc[n][k];
+        for (int n = 0; n < 2 * RT; n++) *reinterpret_cast<float4*>(mine + (n * 32 + lane) * 4) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
       }
       __syncthreads();
       if (ks < h) {
 #pragma unroll
-        for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) acc[n][k] += mine[(n * 4 + k) * 32 + lane];
+        for (int n = 0; n < 2 * RT; n++) {
+          const float4 v = *reinterpret_cast<const float4*>(mine + (n * 32 + lane) * 4);
+          acc[n][0] += v.x;
+          acc[n][1] += v.y;
+          acc[n][2] += v.z;
+          acc[n][3] += v.w;
+        }
       }
       __syncthreads();
     }
@@ -444,11 +507,14 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
 #pragma unroll
       for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) s_part[(16 * wm + i + 8 * (k >> 1)) * RP + 8 * n + 2 * q + (k & 1)] = acc[n][k];
+        for (int h = 0; h < 2; h++)
+          *reinterpret_cast<float2*>(s_part + (16 * wm + i + 8 * h) * RP + 8 * n + 2 * q) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
     }
-    cluster.sync();
+    if (C > 1) cluster.sync();
+    else __syncthreads();
   }
   // u of the whole contraction, saved as bf16 terms and as two terms for the second product. A warp a row at a time.
+#pragma unroll 1
   for (int m = warp; m < MT; m += kThreads / 32) {
     float v[(RP + 31) / 32], most = 0.f;
     const int row = s_row[m];
@@ -458,7 +524,15 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
       v[b] = 0.f;
       if (j < a.r && row >= 0) {
         if (a.shrink) {
-          for (int c = 0; c < C; c++) v[b] += *cluster.map_shared_rank(s_part + m * RP + j, c);
+          if (C == 1) {
+            v[b] = s_part[m * RP + j];
+          } else {
+            float p[8];   // all on their way at once, added in the order of the CTAs
+#pragma unroll
+            for (int c = 0; c < 8; c++) p[c] = c < C ? *cluster.map_shared_rank(s_part + m * RP + j, c) : 0.f;
+#pragma unroll
+            for (int c = 0; c < 8; c++) v[b] += p[c];
+          }
           if (a.scale_u) v[b] *= factor;
         } else {
 #pragma unroll
@@ -500,93 +574,135 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
     if (lane == 0) s_factor[m] = a.scale_u ? f : f * factor;
   }
   __syncthreads();
-  if (a.shrink) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  if (a.shrink && C > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
 
-  const uint32_t u_at = smem_at(s_u);
-  for (int s = n1; s < n1 + n2; s++) {
+  const uint32_t u_at = smem_at(s_u) + ((16 * wm + (lane & 15)) * UP + 8 * (lane >> 4)) * 2;
+  const int cw = CW * ks, m0 = 16 * wm + i;
+  const int row[2] = {s_row[m0], s_row[m0 + 8]};
+  const float f[2] = {s_factor[m0], s_factor[m0 + 8]};
+  // terms of u, in registers where there are not too many
+  constexpr int UK = RT <= 4 ? RT : 1;
+  uint32_t ua[UK][2][4];
+  if constexpr (RT <= 4) {
+#pragma unroll
+    for (int k = 0; k < RT; k++)
+#pragma unroll
+      for (int n = 0; n < 2; n++) ldsm(ua[k][n], u_at + (n * MT * UP + 16 * k) * 2);
+  }
+#pragma unroll 1
+  for (int s = 0; s < n2; s++) {
     cp_wait<S::STAGES - 2>();
     __syncthreads();
-    fetch(s + S::STAGES - 1);
-    const uint32_t at = ring + s % S::STAGES * S::STAGE;
-    const int c0 = lo + (s - n1) * NB, cw = CW * ks;
-    if (16 * wm >= t.rows || c0 + cw >= hi) continue;
-    float acc[CW / 8][4];
+    fetch();
+    const int c0 = lo + s * NB;
+    if (16 * wm < t.rows && c0 + cw < hi) {
+      float acc[CW / 8][4];
 #pragma unroll
-    for (int n = 0; n < CW / 8; n++)
+      for (int n = 0; n < CW / 8; n++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+        for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
 #pragma unroll
-    for (int k = 0; k < RT; k++) {
-      uint32_t ua[2][4];
+      for (int k = 0; k < RT; k++) {
+        if constexpr (RT > 4) {
 #pragma unroll
-      for (int n = 0; n < 2; n++) ldsm(ua[n], u_at + ((n * MT + 16 * wm + (lane & 15)) * UP + 16 * k + 8 * (lane >> 4)) * 2);
-#pragma unroll
-      for (int n = 0; n < CW / 16; n++) {
-        uint32_t b[2][2][P2];
-        load_b<PT, P2, W2C, !BWD>(at + S::Y, cw + 16 * n, 16 * k, b);
-#pragma unroll
-        for (int h = 0; h < 2; h++) mma_terms<2, P2, CT>(acc[2 * n + h], ua, b[h][0], b[h][1]);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int m = 16 * wm + 8 * h + i, row = s_row[m];
-      const float f = s_factor[m];
-      if (a.vec_out && !a.out_f32) {
-        // in the stage's room for the base's rows, from where whole chunks leave
-#pragma unroll
-        for (int n = 0; n < CW / 8; n++) {
-          const uint32_t p = YTile::at(at, m, cw / 8 + n) + 4 * q;
-          float y0 = 0.f, y1 = 0.f;
-          if (staged) {
-            uint32_t v;
-            asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(p) : "memory");
-            const XT* y = reinterpret_cast<const XT*>(&v);
-            y0 = to_float(y[0]);
-            y1 = to_float(y[1]);
-          }
-          XT o[2] = {XT(fmaf(f, acc[n][2 * h], y0)), XT(fmaf(f, acc[n][2 * h + 1], y1))};
-          asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(p), "r"(*reinterpret_cast<const uint32_t*>(o)) : "memory");
+          for (int n = 0; n < 2; n++) ldsm(ua[0][n], u_at + (n * MT * UP + 16 * k) * 2);
         }
-      } else if (row >= 0) {
 #pragma unroll
-        for (int n = 0; n < CW / 8; n++)
+        for (int n = 0; n < CW / 16; n++) {
+          uint32_t b[2][2][P2];
+          load_b<PT, P2, W2C, !BWD>(at + S::Y, cw + 16 * n, 16 * k, b);
 #pragma unroll
-          for (int k = 0; k < 2; k++) {
-            const int col = c0 + cw + 8 * n + 2 * q + k;
-            if (col >= hi) continue;
-            if (a.out_f32) {
-              static_cast<float*>(a.out)[(long long)row * a.out_stride + col - a.c0] = f * acc[n][2 * h + k];
-            } else {
-              const float y = a.base != nullptr ? to_float(static_cast<const XT*>(a.base)[(long long)row * a.base_stride + col]) : 0.f;
-              static_cast<XT*>(a.out)[(long long)row * a.out_stride + col] = XT(fmaf(f, acc[n][2 * h + k], y));
+          for (int h = 0; h < 2; h++) mma_terms<2, P2, CT>(acc[2 * n + h], ua[RT > 4 ? 0 : k], b[h][0], b[h][1]);
+        }
+      }
+      if constexpr (!BWD) {
+        // columns c0 + cw + (CW / 4) q .. of two rows
+        constexpr int HOLD = CW / 4;
+        const int col = c0 + cw + HOLD * q;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          if (a.vec_out) {
+            if (row[h] < 0 || col >= hi) continue;
+            uint32_t v[HOLD / 2];
+            const uint32_t p = YTile::at(at, m0 + 8 * h, (cw + HOLD * q) / 8) + (HOLD == 4 ? 8 * (q & 1) : 0);
+            if constexpr (HOLD == 8) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(p) : "memory");
+            else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];\n" : "=r"(v[0]), "=r"(v[1]) : "r"(p) : "memory");
+            XT* y = reinterpret_cast<XT*>(v);
+#pragma unroll
+            for (int n = 0; n < HOLD / 2; n++) {
+              y[2 * n] = XT(fmaf(f[h], acc[n][2 * h], to_float(y[2 * n])));
+              y[2 * n + 1] = XT(fmaf(f[h], acc[n][2 * h + 1], to_float(y[2 * n + 1])));
             }
-          }
-      }
-    }
-    if (a.vec_out && !a.out_f32) {
-      __syncwarp();
-      constexpr int EACH = CW / 8;   // chunks of a row
+            XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride + col;
+            if constexpr (HOLD == 8) *reinterpret_cast<uint4*>(o) = make_uint4(v[0], v[1], v[2], v[3]);
+            else *reinterpret_cast<uint2*>(o) = make_uint2(v[0], v[1]);
+          } else if (row[h] >= 0) {
+            const XT* y = static_cast<const XT*>(a.base) + (long long)row[h] * a.base_stride;
+            XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride;
 #pragma unroll
-      for (int c = lane; c < 16 * EACH; c += 32) {
-        const int m = 16 * wm + c / EACH, ch = cw / 8 + c % EACH, row = s_row[m], col = c0 + 8 * ch;
-        if (row < 0 || col >= hi) continue;
-        uint4 v;
-        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(YTile::at(at, m, ch)) : "memory");
-        *reinterpret_cast<uint4*>(static_cast<XT*>(a.out) + (long long)row * a.out_stride + col) = v;
+            for (int n = 0; n < HOLD; n++)
+              if (col + n < hi) o[col + n] = XT(fmaf(f[h], acc[n / 2][2 * h + n % 2], to_float(y[col + n])));
+          }
+        }
+      } else if (a.out_f32) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          if (row[h] < 0) continue;
+          float* o = static_cast<float*>(a.out) + (long long)row[h] * a.out_stride - a.c0;
+#pragma unroll
+          for (int n = 0; n < CW / 8; n++) {
+            const int col = c0 + cw + 8 * n + 2 * q;
+            if (a.out_stride % 2 == 0 && col + 1 < hi) *reinterpret_cast<float2*>(o + col) = make_float2(f[h] * acc[n][2 * h], f[h] * acc[n][2 * h + 1]);
+            else
+#pragma unroll
+              for (int k = 0; k < 2; k++)
+                if (col + k < hi) o[col + k] = f[h] * acc[n][2 * h + k];
+          }
+        }
+      } else if (a.vec_out) {
+        // through the stage's room for rows, from where whole chunks leave
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int n = 0; n < CW / 8; n++) {
+            const XT o[2] = {XT(f[h] * acc[n][2 * h]), XT(f[h] * acc[n][2 * h + 1])};
+            asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(YTile::at(at, m0 + 8 * h, cw / 8 + n) + 4 * q), "r"(*reinterpret_cast<const uint32_t*>(o)) : "memory");
+          }
+        __syncwarp();
+        constexpr int EACH = CW / 8;   // chunks of a row
+#pragma unroll
+        for (int c = lane; c < 16 * EACH; c += 32) {
+          const int m = 16 * wm + c / EACH, ch = cw / 8 + c % EACH, e = s_row[m], col = c0 + 8 * ch;
+          if (e < 0 || col >= hi) continue;
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(YTile::at(at, m, ch)) : "memory");
+          *reinterpret_cast<uint4*>(static_cast<XT*>(a.out) + (long long)e * a.out_stride + col) = v;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          if (row[h] < 0) continue;
+          XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride;
+#pragma unroll
+          for (int n = 0; n < CW / 8; n++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+              if (c0 + cw + 8 * n + 2 * q + k < hi) o[c0 + cw + 8 * n + 2 * q + k] = XT(f[h] * acc[n][2 * h + k]);
+        }
       }
     }
+    advance();
   }
   cp_wait<0>();
   // nobody leaves while its part of u may still be read
   __syncthreads();
-  if (a.shrink) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  if (a.shrink && C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
-template <typename XT, typename PT, bool BWD, int RT, int MT>
+template <typename XT, typename PT, bool BWD, int RT, int MT, bool FAST>
 cudaError_t launch_tile(const LoraArgs& a, int cluster, cudaStream_t st) {
   constexpr int smem = Shape<PT, BWD, RT, MT>::SMEM;
-  auto kern = tile_kernel<XT, PT, BWD, RT, MT>;
+  auto kern = tile_kernel<XT, PT, BWD, RT, MT, FAST>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
@@ -605,7 +721,9 @@ cudaError_t launch_tile(const LoraArgs& a, int cluster, cudaStream_t st) {
 }
 template <typename XT, typename PT, bool BWD, int RT>
 cudaError_t launch_mt(const LoraArgs& a, int mt, int cluster, cudaStream_t st) {
-  return mt == 16 ? launch_tile<XT, PT, BWD, RT, 16>(a, cluster, st) : launch_tile<XT, PT, BWD, RT, 64>(a, cluster, st);
+  if (a.by_in == kBy16 && a.by_w1 == kBy16 && a.by_w2 == kBy16)
+    return mt == 16 ? launch_tile<XT, PT, BWD, RT, 16, true>(a, cluster, st) : launch_tile<XT, PT, BWD, RT, 64, true>(a, cluster, st);
+  return mt == 16 ? launch_tile<XT, PT, BWD, RT, 16, false>(a, cluster, st) : launch_tile<XT, PT, BWD, RT, 64, false>(a, cluster, st);
 }
 template <typename XT, typename PT, bool BWD>
 cudaError_t launch_rt(const LoraArgs& a, int mt, int cluster, cudaStream_t st) {
