@@ -70,6 +70,11 @@ __device__ __forceinline__ uint32_t round_bf16(float f0, float f1) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(f0, f1);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ uint32_t round_pair(float f0, float f1, bf16) { return round_bf16(f0, f1); }
+__device__ __forceinline__ uint32_t round_pair(float f0, float f1, __half) {
+  const __half2 v = __floats2half2_rn(f0, f1);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 // The leading bits of two floats as a bf16 pair, cut off (never rounded up to infinity), and what is left of them: of an infinity
 // nothing.
 __device__ __forceinline__ uint32_t take_bf16(float& f0, float& f1) {
@@ -286,19 +291,24 @@ __device__ __forceinline__ void copy_rows(const LoraArgs& a, const int* s_row, i
 // ---------------------------------------------------------------------------------------------------- both products
 template <typename PT, bool BWD, int RT, int MT>
 struct Shape {
-  static constexpr int RP = 16 * RT, PS = sizeof(PT), WM = MT / 16, KS = kThreads / 32 / WM;   // KS warps share sixteen rows
-  static constexpr int KB = MT == 64 ? 64 : 128;                 // contraction of a stage of the first product
-  static constexpr int CW = MT == 64 ? 32 : 16, NB = CW * KS;    // columns of a warp and of a stage of the second
+  static constexpr int RP = 16 * RT, PS = sizeof(PT);
+  // A warp has MW sixteens of rows, so that a weight fragment (and the split of a float32 one) serves all of them; KS warps share
+  // their contraction. float32, 4096 rows, K 4096, N 14336, rank 16: MW 1, 2, 4 forward 86, 75, 80 us, backward 84, 67, 62.
+  static constexpr int MW = MT == 16 ? 1 : PS == 4 ? (RT == 8 ? 1 : RT == 4 || !BWD ? 2 : 4) : RT >= 4 ? 1 : 2, WM = MT / 16 / MW, KS = kThreads / 32 / WM;
+  static constexpr int KB = MT == 16 ? (RT <= 2 && PS == 2 ? 256 : 128) : RT <= 2 ? 128 : 64;   // contraction of a stage of the first product
+  static constexpr int CW = MT == 16 ? (RT <= 2 && PS == 2 ? 32 : 16) : KS == 8 || RT == 4 && PS == 4 ? 16 : 32;   // columns of a warp in a stage of the second
+  static constexpr int NB = CW * KS;
   static constexpr int X = MT * KB * 2, W1 = RP * KB * PS, Y = MT * NB * 2, W2 = NB * RP * PS;
   static constexpr int STAGE = X + W1 > Y + W2 ? X + W1 : Y + W2;
   static constexpr int UP = RP + 8;
-  // the sums of half of the warps, and then the CTA's part of u, in one place
-  static constexpr int RED = KS / 2 * WM * 16 * RP * 4, PART = MT * RP * 4, SUM = RED > PART ? RED : PART, U = 2 * MT * UP * 2;
+  // room for the sums of some of the warps, and then for the CTA's part of u, in one place
+  static constexpr int SLOTS = MT == 16 ? 4 : KS == 8 ? 2 : 1, SLOT = 16 * MW * RP;
+  static constexpr int RED = SLOTS * WM * SLOT * 4, PART = MT * RP * 4, SUM = RED > PART ? RED : PART, U = 2 * MT * UP * 2;
   static constexpr int REST = SUM + U + MT * 8 + 16;
-  // two CTAs of an SM where at least four stages of each fit, else one
+  // two CTAs of an SM where at least three stages of each fit, else one
   static constexpr int TWO = (112 * 1024 - REST) / STAGE, ONE = (224 * 1024 - REST) / STAGE;
-  static constexpr int STAGES = TWO >= 4 ? (TWO > 8 ? 8 : TWO) : ONE > 6 ? 6 : ONE;
-  static constexpr int SMEM = STAGES * STAGE + REST;
+  static constexpr int STAGES = TWO >= 3 ? (TWO > 8 ? 8 : TWO) : ONE > 6 ? 6 : ONE;
+  static constexpr int SMEM = STAGES * STAGE + REST, CTAS = TWO >= 3 ? 2 : 1;
   static_assert(STAGES >= 2 && SMEM <= 227 * 1024, "does not fit");
 };
 
@@ -324,10 +334,10 @@ __device__ __forceinline__ int place_of(int n) {
 
 // FAST: all rows are whole aligned groups of 16 bytes.
 template <typename XT, typename PT, bool BWD, int RT, int MT, bool FAST>
-__global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_kernel(const LoraArgs a) {
   typedef Shape<PT, BWD, RT, MT> S;
   typedef typename std::conditional<sizeof(PT) == 4, bf16, XT>::type CT;
-  constexpr int RP = S::RP, UP = S::UP, KS = S::KS, WM = S::WM, KB = S::KB, NB = S::NB, CW = S::CW, PS = S::PS;
+  constexpr int RP = S::RP, UP = S::UP, KS = S::KS, WM = S::WM, MW = S::MW, KB = S::KB, NB = S::NB, CW = S::CW, PS = S::PS;
   constexpr int XN = RowTerms<XT, CT>::N, P1 = PS == 4 ? 3 : 1, P2 = PS == 4 ? 2 : 1, UT = PS == 4 ? 3 : 2;
   constexpr int W1C = BWD ? RP : KB, W2C = BWD ? NB : RP;   // columns of the stages' weight tiles
   typedef Deal<MT, KB, 2> XD;
@@ -346,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, q = lane & 3;
-  const int wm = warp % WM, ks = warp / WM;
+  const int m0 = warp % WM * 16 * MW, ks = warp / WM;   // the warp's first row, its share of the others' work
   const TileAt t = find_tile<MT>(a, blockIdx.x / C, s_row, s_info);
   if (t.rows == 0) return;   // (the whole cluster)
   const int n_chunks = (a.c1 - a.c0 + NB - 1) / NB;
@@ -438,77 +448,90 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
   auto advance = [&]() { at = at + S::STAGE == ring + S::STAGES * S::STAGE ? ring : at + S::STAGE; };
 
   if (a.shrink) {
-    float acc[2 * RT][4];
+    float acc[MW][2 * RT][4];
 #pragma unroll
-    for (int n = 0; n < 2 * RT; n++)
+    for (int m = 0; m < MW; m++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+      for (int n = 0; n < 2 * RT; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc[m][n][k] = 0.f;
 #pragma unroll 1
     for (int s = 0; s < n1; s++) {
       cp_wait<S::STAGES - 2>();
       __syncthreads();
       fetch();
-      // The tensor cores cut off what a sum has below its last bit. Where float32 results are wanted, a stage's products are added up
-      // by themselves and then, rounded, to the whole.
-      float part[2 * RT][4];
-      if constexpr (PS == 4) {
-#pragma unroll
-        for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) part[n][k] = 0.f;
-      }
 #pragma unroll
       for (int k = 0; k < KB / 16 / KS; k++) {
         const int step = ks + k * KS;
-        uint32_t raw[4], xa[XN][4];
-        ldsm(raw, XTile::at(at, 16 * wm + (lane & 15), 2 * step + (lane >> 4)));
-        RowTerms<XT, CT>::get(raw, xa);
+        uint32_t xa[MW][XN][4];
+#pragma unroll
+        for (int m = 0; m < MW; m++) {
+          if (m > 0 && m0 + 16 * m >= t.rows) break;
+          uint32_t raw[4];
+          ldsm(raw, XTile::at(at, m0 + 16 * m + (lane & 15), 2 * step + (lane >> 4)));
+          RowTerms<XT, CT>::get(raw, xa[m]);
+        }
 #pragma unroll
         for (int n = 0; n < RT; n++) {
           uint32_t b[2][2][P1];
           load_b<PT, P1, W1C, !BWD>(at + S::X, 16 * n, 16 * step, b);
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            if constexpr (PS == 4) mma_terms<XN, P1, CT>(part[2 * n + h], xa, b[h][0], b[h][1]);
-            else mma_terms<XN, P1, CT>(acc[2 * n + h], xa, b[h][0], b[h][1]);
+          for (int m = 0; m < MW; m++) {
+            if (m > 0 && m0 + 16 * m >= t.rows) break;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              if constexpr (PS == 4) {
+                // The tensor cores cut off what a sum has below its last bit. Where float32 results are wanted, a step's products
+                // are added up by themselves and then, rounded, to the whole.
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_terms<XN, P1, CT>(part, xa[m], b[h][0], b[h][1]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[m][2 * n + h][c] += part[c];
+              } else {
+                mma_terms<XN, P1, CT>(acc[m][2 * n + h], xa[m], b[h][0], b[h][1]);
+              }
+            }
           }
         }
       }
-      if constexpr (PS == 4) {
+      advance();
+    }
+    // the warps' parts, halves onto halves, as many at a time as there is room for
+#pragma unroll
+    for (int h = KS / 2; h > 0; h >>= 1)
+#pragma unroll
+      for (int b = 0; b < h; b += S::SLOTS) {
+        float* mine = s_red + (warp % WM * S::SLOTS + (ks >= h ? ks - h - b : ks - b)) * S::SLOT;
+        if (ks >= h + b && ks < h + b + S::SLOTS && ks < 2 * h) {
+#pragma unroll
+          for (int m = 0; m < MW; m++)
+#pragma unroll
+            for (int n = 0; n < 2 * RT; n++)
+              *reinterpret_cast<float4*>(mine + ((m * 2 * RT + n) * 32 + lane) * 4) = make_float4(acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]);
+        }
+        __syncthreads();
+        if (ks >= b && ks < b + S::SLOTS && ks < h) {
+#pragma unroll
+          for (int m = 0; m < MW; m++)
+#pragma unroll
+            for (int n = 0; n < 2 * RT; n++) {
+              const float4 v = *reinterpret_cast<const float4*>(mine + ((m * 2 * RT + n) * 32 + lane) * 4);
+              acc[m][n][0] += v.x;
+              acc[m][n][1] += v.y;
+              acc[m][n][2] += v.z;
+              acc[m][n][3] += v.w;
+            }
+        }
+        __syncthreads();
+      }
+    if (ks == 0) {
+#pragma unroll
+      for (int m = 0; m < MW; m++)
 #pragma unroll
         for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) acc[n][k] += part[n][k];
-      }
-      advance();
-    }
-    // the warps' parts, halves onto halves
-#pragma unroll
-    for (int h = KS / 2; h > 0; h >>= 1) {
-      float* mine = s_red + (wm * (KS / 2) + ks % h) * 16 * RP;
-      if (ks >= h && ks < 2 * h) {
-#pragma unroll
-        for (int n = 0; n < 2 * RT; n++) *reinterpret_cast<float4*>(mine + (n * 32 + lane) * 4) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-      }
-      __syncthreads();
-      if (ks < h) {
-#pragma unroll
-        for (int n = 0; n < 2 * RT; n++) {
-          const float4 v = *reinterpret_cast<const float4*>(mine + (n * 32 + lane) * 4);
-          acc[n][0] += v.x;
-          acc[n][1] += v.y;
-          acc[n][2] += v.z;
-          acc[n][3] += v.w;
-        }
-      }
-      __syncthreads();
-    }
-    if (ks == 0) {
-#pragma unroll
-      for (int n = 0; n < 2 * RT; n++)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-          *reinterpret_cast<float2*>(s_part + (16 * wm + i + 8 * h) * RP + 8 * n + 2 * q) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+          for (int h = 0; h < 2; h++)
+            *reinterpret_cast<float2*>(s_part + (m0 + 16 * m + i + 8 * h) * RP + 8 * n + 2 * q) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
     }
     if (C > 1) cluster.sync();
     else __syncthreads();
@@ -576,118 +599,114 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const LoraArgs a) {
   __syncthreads();
   if (a.shrink && C > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
 
-  const uint32_t u_at = smem_at(s_u) + ((16 * wm + (lane & 15)) * UP + 8 * (lane >> 4)) * 2;
-  const int cw = CW * ks, m0 = 16 * wm + i;
-  const int row[2] = {s_row[m0], s_row[m0 + 8]};
-  const float f[2] = {s_factor[m0], s_factor[m0 + 8]};
-  // terms of u, in registers where there are not too many
-  constexpr int UK = RT <= 4 ? RT : 1;
-  uint32_t ua[UK][2][4];
-  if constexpr (RT <= 4) {
-#pragma unroll
-    for (int k = 0; k < RT; k++)
-#pragma unroll
-      for (int n = 0; n < 2; n++) ldsm(ua[k][n], u_at + (n * MT * UP + 16 * k) * 2);
-  }
+  const uint32_t u_at = smem_at(s_u) + ((m0 + (lane & 15)) * UP + 8 * (lane >> 4)) * 2;
+  const int cw = CW * ks;
 #pragma unroll 1
   for (int s = 0; s < n2; s++) {
     cp_wait<S::STAGES - 2>();
     __syncthreads();
     fetch();
     const int c0 = lo + s * NB;
-    if (16 * wm < t.rows && c0 + cw < hi) {
-      float acc[CW / 8][4];
+    if (m0 < t.rows && c0 + cw < hi) {
+      float acc[MW][CW / 8][4];
 #pragma unroll
-      for (int n = 0; n < CW / 8; n++)
+      for (int m = 0; m < MW; m++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+        for (int n = 0; n < CW / 8; n++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) acc[m][n][k] = 0.f;
 #pragma unroll
       for (int k = 0; k < RT; k++) {
-        if constexpr (RT > 4) {
+        uint32_t b[CW / 16][2][2][P2];
 #pragma unroll
-          for (int n = 0; n < 2; n++) ldsm(ua[0][n], u_at + (n * MT * UP + 16 * k) * 2);
-        }
+        for (int n = 0; n < CW / 16; n++) load_b<PT, P2, W2C, !BWD>(at + S::Y, cw + 16 * n, 16 * k, b[n]);
 #pragma unroll
-        for (int n = 0; n < CW / 16; n++) {
-          uint32_t b[2][2][P2];
-          load_b<PT, P2, W2C, !BWD>(at + S::Y, cw + 16 * n, 16 * k, b);
+        for (int m = 0; m < MW; m++) {
+          if (m > 0 && m0 + 16 * m >= t.rows) break;
+          uint32_t ua[2][4];
 #pragma unroll
-          for (int h = 0; h < 2; h++) mma_terms<2, P2, CT>(acc[2 * n + h], ua[RT > 4 ? 0 : k], b[h][0], b[h][1]);
+          for (int n = 0; n < 2; n++) ldsm(ua[n], u_at + ((n * MT + 16 * m) * UP + 16 * k) * 2);
+#pragma unroll
+          for (int n = 0; n < CW / 8; n++) mma_terms<2, P2, CT>(acc[m][n], ua, b[n / 2][n % 2][0], b[n / 2][n % 2][1]);
         }
       }
-      if constexpr (!BWD) {
-        // columns c0 + cw + (CW / 4) q .. of two rows
-        constexpr int HOLD = CW / 4;
-        const int col = c0 + cw + HOLD * q;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          if (a.vec_out) {
+      for (int m = 0; m < MW; m++) {
+        if (m > 0 && m0 + 16 * m >= t.rows) break;
+        const int m1 = m0 + 16 * m + i;
+        const int row[2] = {s_row[m1], s_row[m1 + 8]};
+        const float f[2] = {s_factor[m1], s_factor[m1 + 8]};
+        if constexpr (!BWD) {
+          // columns c0 + cw + (CW / 4) q .. of two rows
+          constexpr int HOLD = CW / 4;
+          const int col = c0 + cw + HOLD * q;
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
             if (row[h] < 0 || col >= hi) continue;
-            uint32_t v[HOLD / 2];
-            const uint32_t p = YTile::at(at, m0 + 8 * h, (cw + HOLD * q) / 8) + (HOLD == 4 ? 8 * (q & 1) : 0);
-            if constexpr (HOLD == 8) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(p) : "memory");
-            else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];\n" : "=r"(v[0]), "=r"(v[1]) : "r"(p) : "memory");
-            XT* y = reinterpret_cast<XT*>(v);
-#pragma unroll
-            for (int n = 0; n < HOLD / 2; n++) {
-              y[2 * n] = XT(fmaf(f[h], acc[n][2 * h], to_float(y[2 * n])));
-              y[2 * n + 1] = XT(fmaf(f[h], acc[n][2 * h + 1], to_float(y[2 * n + 1])));
-            }
+            const float (&c)[CW / 8][4] = acc[m];
             XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride + col;
-            if constexpr (HOLD == 8) *reinterpret_cast<uint4*>(o) = make_uint4(v[0], v[1], v[2], v[3]);
-            else *reinterpret_cast<uint2*>(o) = make_uint2(v[0], v[1]);
-          } else if (row[h] >= 0) {
-            const XT* y = static_cast<const XT*>(a.base) + (long long)row[h] * a.base_stride;
+            if (a.vec_out) {
+              uint32_t v[HOLD / 2];
+              const uint32_t p = YTile::at(at, m1 + 8 * h, (cw + HOLD * q) / 8) + (HOLD == 4 ? 8 * (q & 1) : 0);
+              if constexpr (HOLD == 8) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(p) : "memory");
+              else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];\n" : "=r"(v[0]), "=r"(v[1]) : "r"(p) : "memory");
+#pragma unroll
+              for (int n = 0; n < HOLD / 2; n++) {
+                const XT* y = reinterpret_cast<const XT*>(&v[n]);
+                v[n] = round_pair(fmaf(f[h], c[n][2 * h], to_float(y[0])), fmaf(f[h], c[n][2 * h + 1], to_float(y[1])), XT());
+              }
+              if constexpr (HOLD == 8) *reinterpret_cast<uint4*>(o) = make_uint4(v[0], v[1], v[2], v[3]);
+              else *reinterpret_cast<uint2*>(o) = make_uint2(v[0], v[1]);
+            } else {
+              const XT* y = static_cast<const XT*>(a.base) + (long long)row[h] * a.base_stride + col;
+#pragma unroll
+              for (int n = 0; n < HOLD; n++)
+                if (col + n < hi) o[n] = XT(fmaf(f[h], c[n / 2][2 * h + n % 2], to_float(y[n])));
+            }
+          }
+        } else if (a.out_f32) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if (row[h] < 0) continue;
+            float* o = static_cast<float*>(a.out) + (long long)row[h] * a.out_stride - a.c0;
+#pragma unroll
+            for (int n = 0; n < CW / 8; n++) {
+              const int col = c0 + cw + 8 * n + 2 * q;
+              if (a.out_stride % 2 == 0 && col + 1 < hi) *reinterpret_cast<float2*>(o + col) = make_float2(f[h] * acc[m][n][2 * h], f[h] * acc[m][n][2 * h + 1]);
+              else
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                  if (col + k < hi) o[col + k] = f[h] * acc[m][n][2 * h + k];
+            }
+          }
+        } else if (a.vec_out) {
+          // through the stage's room for rows, from where whole chunks leave
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int n = 0; n < CW / 8; n++)
+              asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(YTile::at(at, m1 + 8 * h, cw / 8 + n) + 4 * q), "r"(round_pair(f[h] * acc[m][n][2 * h], f[h] * acc[m][n][2 * h + 1], XT())) : "memory");
+          __syncwarp();
+          constexpr int EACH = CW / 8;   // chunks of a row
+#pragma unroll
+          for (int c = lane; c < 16 * EACH; c += 32) {
+            const int mr = m0 + 16 * m + c / EACH, ch = cw / 8 + c % EACH, e = s_row[mr], col = c0 + 8 * ch;
+            if (e < 0 || col >= hi) continue;
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(YTile::at(at, mr, ch)) : "memory");
+            *reinterpret_cast<uint4*>(static_cast<XT*>(a.out) + (long long)e * a.out_stride + col) = v;
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if (row[h] < 0) continue;
             XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride;
 #pragma unroll
-            for (int n = 0; n < HOLD; n++)
-              if (col + n < hi) o[col + n] = XT(fmaf(f[h], acc[n / 2][2 * h + n % 2], to_float(y[col + n])));
-          }
-        }
-      } else if (a.out_f32) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          if (row[h] < 0) continue;
-          float* o = static_cast<float*>(a.out) + (long long)row[h] * a.out_stride - a.c0;
-#pragma unroll
-          for (int n = 0; n < CW / 8; n++) {
-            const int col = c0 + cw + 8 * n + 2 * q;
-            if (a.out_stride % 2 == 0 && col + 1 < hi) *reinterpret_cast<float2*>(o + col) = make_float2(f[h] * acc[n][2 * h], f[h] * acc[n][2 * h + 1]);
-            else
+            for (int n = 0; n < CW / 8; n++)
 #pragma unroll
               for (int k = 0; k < 2; k++)
-                if (col + k < hi) o[col + k] = f[h] * acc[n][2 * h + k];
+                if (c0 + cw + 8 * n + 2 * q + k < hi) o[c0 + cw + 8 * n + 2 * q + k] = XT(f[h] * acc[m][n][2 * h + k]);
           }
-        }
-      } else if (a.vec_out) {
-        // through the stage's room for rows, from where whole chunks leave
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int n = 0; n < CW / 8; n++) {
-            const XT o[2] = {XT(f[h] * acc[n][2 * h]), XT(f[h] * acc[n][2 * h + 1])};
-            asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(YTile::at(at, m0 + 8 * h, cw / 8 + n) + 4 * q), "r"(*reinterpret_cast<const uint32_t*>(o)) : "memory");
-          }
-        __syncwarp();
-        constexpr int EACH = CW / 8;   // chunks of a row
-#pragma unroll
-        for (int c = lane; c < 16 * EACH; c += 32) {
-          const int m = 16 * wm + c / EACH, ch = cw / 8 + c % EACH, e = s_row[m], col = c0 + 8 * ch;
-          if (e < 0 || col >= hi) continue;
-          uint4 v;
-          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(YTile::at(at, m, ch)) : "memory");
-          *reinterpret_cast<uint4*>(static_cast<XT*>(a.out) + (long long)e * a.out_stride + col) = v;
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          if (row[h] < 0) continue;
-          XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride;
-#pragma unroll
-          for (int n = 0; n < CW / 8; n++)
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-              if (c0 + cw + 8 * n + 2 * q + k < hi) o[c0 + cw + 8 * n + 2 * q + k] = XT(f[h] * acc[n][2 * h + k]);
         }
       }
     }
