@@ -5,11 +5,14 @@
 // these the top_k largest q are picked, lowest index first among equals, groups and experts alike. Weights
 // w_j = scale * s_ij / (sum s_i + 1e-20), or scale * s_ij.
 //
-// A warp per token, a lane NI neighbouring experts, all in registers. The order is that of 64 bits, but sums in 64 bits of
-// exponentials in 64 bits took 66 us for 16384 tokens of 256 experts. So the kernel ranks floats first, whose error is bounded
-// (kRouteSlack): where the neighbours in the order of the picks, the last of them and the best that is left, and the groups around the
-// border lie further apart than that, 64 bits would give the same order; where they don't, unless they are bit for bit the same
-// logit and bias, the token is ranked again in 64 bits. Logits alone need neither: they are compared as they are.
+// A warp per token, a lane NI neighbouring experts, all in registers. The order is that of 64 bits; exponentials and sums in 64 bits
+// for all experts took 66 us for 16384 tokens of 256 experts, this kernel takes 13. It ranks 32-bit codes: what an expert is ranked
+// by in the upper bits (score + bias as fixed point over the range of the biases, or a logit's leading bits), its index, counted
+// down, in the lower ones. A lane sorts its codes, and each pick is one warp-wide maximum of the lanes' first. The codes' error is
+// bounded (kRouteSlack): where neighbours in the order of the picks, the last of them and the best that is left, or the sums around the
+// border of the groups lie no further apart than that, and are not the same logit and bias bit for bit, the token is ranked again in
+// 64 bits. A code holds all of a 16-bit logit: without a bias and sums nothing is ever ranked again. What is left is instruction
+// issue: some 450 a token.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -47,15 +50,9 @@ __device__ __forceinline__ uint32_t rt_order(float f) {
   const uint32_t b = __float_as_uint(f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float rt_unorder(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 
-// The largest of the lanes' values and the lowest index that has it: a reduction of the whole warp in one instruction each.
-__device__ __forceinline__ float rt_best(float v, int e, int& best) {
-  const uint32_t mine = rt_order(v + 0.f), most = __reduce_max_sync(kAll, mine);   // (a negative zero is equal to zero)
-  best = (int)__reduce_min_sync(kAll, mine == most ? (uint32_t)e : 0x7fffffffu);
-  return rt_unorder(most);
-}
-__device__ __forceinline__ double rt_best(double v, int e, int& best) {
+// the largest of the lanes' values, and the lowest index that has it
+__device__ __forceinline__ void rt_best(double v, int e, int& best) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const double ov = __shfl_xor_sync(kAll, v, o);
@@ -66,12 +63,11 @@ __device__ __forceinline__ double rt_best(double v, int e, int& best) {
     }
   }
   best = e;
-  return v;
 }
 
-// Error of a float score + bias, relative to 1 + |bias| (scores are at most 1): expf, the sum of up to 1024 exponentials (32 a lane
-// and five steps of a tree, each step half a last bit of what is there), the quotient and the sum with the bias are off by less
-// than 48 halves of a step.
+// Error of a float score + bias, relative to 1 + |bias| (scores are at most 1): the exponential and the quotient in their fast forms
+// (2 + 1.16 |x| and 2 steps, the former weighted with s (1 - s)), the sum of up to 1024 exponentials (32 a lane and five steps of
+// a tree, half a last bit each) and the sum with the bias are off by less than 48 halves of a step.
 constexpr float kRouteSlack = 48.f * 0x1p-24f;
 
 // the lane's NI logits, -infinity where there are none
@@ -186,15 +182,13 @@ __device__ __forceinline__ void drop_groups(const RouteArgs& a, const uint32_t* 
   }
 }
 
-// The top_k largest keys, lowest index first among equals; lane r returns the r-th, -1 where none is left. With a slack: `close` is set,
-// and the picks are void, where neighbours in the order lie within it and are not the same logit and bias in every bit.
-template <typename T, typename K, int NI>
-__device__ __forceinline__ int pick(const RouteArgs& a, const T* row, K (&key)[NI], const float (&l)[NI], const float (&bias)[NI], K slack, bool& close) {
+// The top_k largest keys, lowest index first among equals; lane r returns the r-th, -1 where none is left.
+template <int NI>
+__device__ __forceinline__ int pick(const RouteArgs& a, double (&key)[NI]) {
   const int lane = threadIdx.x & 31, e0 = NI * lane;
-  int win = -1, before = 0;
-  K last = 0;
+  int win = -1;
   for (int r = 0; r < a.top_k; r++) {
-    K bv = -INFINITY;
+    double bv = -INFINITY;
     int be = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < NI; i++)
@@ -203,111 +197,37 @@ __device__ __forceinline__ int pick(const RouteArgs& a, const T* row, K (&key)[N
         be = e0 + i;
       }
     int best;
-    const K top = rt_best(bv, be, best);
+    rt_best(bv, be, best);
     if (best >= a.E) return win;   // no expert is left
-    if (slack > 0 && r > 0 && !(last - top > slack) &&
-        !(static_cast<float>(row[best]) == static_cast<float>(row[before]) && a.bias[best] == a.bias[before])) {
-      close = true;
-      return win;
-    }
 #pragma unroll
     for (int i = 0; i < NI; i++)
       if (e0 + i == best) key[i] = -INFINITY;
-    last = top;
-    before = best;
     if (lane == r) win = best;
-  }
-  if (slack > 0) {
-    // the best of what is left and not the last pick's equal
-    const float ll = static_cast<float>(row[before]), lb = a.bias[before];
-    K bv = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NI; i++)
-      if (!(l[i] == ll && bias[i] == lb) && key[i] > bv) bv = key[i];
-    close = __any_sync(kAll, bv > -INFINITY && !(last - bv > slack));
   }
   return win;
 }
 
-template <typename T, int NI>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs a) {
-  extern __shared__ double route_smem[];   // per warp, with groups: what they count, E keys, bits
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int token = blockIdx.x * kRouteWarps + warp;
-  if (token >= a.T) return;
-  double* grp = route_smem + (size_t)warp * (a.G + a.E + 16);
-  uint32_t* bits = reinterpret_cast<uint32_t*>(grp + a.G + a.E);
-  const T* row = static_cast<const T*>(a.logits) + (long long)token * a.E;
-  const int e0 = NI * lane;
-  float l[NI], key[NI], bias[NI];
-  load_row<T, NI>(row, a.E, a.whole, l);
+__device__ __forceinline__ float rt_first(float x) { return x == x ? x : INFINITY; }   // NaN comes first, so that it is seen
+
+// softmax: the largest logit, and the sum of the exponentials, which replace the logits' in s
+template <int NI>
+__device__ __forceinline__ void softmax(const float (&l)[NI], float (&s)[NI], float& fm, float& fz) {
+  float m = -INFINITY, z = 0.f;
 #pragma unroll
-  for (int i = 0; i < NI; i++) bias[i] = a.bias != nullptr && e0 + i < a.E ? a.bias[e0 + i] : 0.f;
-  float fm = 0.f, fz = 1.f;   // softmax: the largest logit, the sum of exponentials
-  if (a.scoring == 0) {
-    float m = -INFINITY, s = 0.f;
+  for (int i = 0; i < NI; i++) m = fmaxf(m, l[i]);
+  fm = rt_max(m);
 #pragma unroll
-    for (int i = 0; i < NI; i++) m = fmaxf(m, l[i]);
-    fm = rt_max(m);
-#pragma unroll
-    for (int i = 0; i < NI; i++) s += l[i] == -INFINITY ? 0.f : expf(l[i] - fm);
-    fz = rt_sum(s);
+  for (int i = 0; i < NI; i++) {
+    s[i] = l[i] == -INFINITY ? 0.f : expf(l[i] - fm);
+    z += s[i];
   }
-  // what experts are ranked by, and groups
-  const bool by_score = a.bias != nullptr, groups_by_score = by_score || a.group_top > 1;
-  auto by_logit = [&](float x) { return x == x ? x : INFINITY; };   // NaN comes first, so that it is seen
-  float slack = kRouteSlack;
-  if (by_score || (a.G > 1 && groups_by_score)) {
-    float most = 0.f;
-#pragma unroll
-    for (int i = 0; i < NI; i++) {
-      const float q = (a.scoring == 0 ? expf(l[i] - fm) / fz : rt_sigmoid(l[i])) + bias[i];
-      key[i] = l[i] == -INFINITY ? -INFINITY : by_logit(q);
-      if (fabsf(bias[i]) < INFINITY) most = fmaxf(most, fabsf(bias[i]));
-    }
-    if (by_score) slack *= 1.f + rt_max(most);
-  } else {
-#pragma unroll
-    for (int i = 0; i < NI; i++) key[i] = by_logit(l[i]);
-  }
-  bool close = false;
-  int win = -1;
-  if (a.G > 1) {
-    float* g32 = reinterpret_cast<float*>(grp);
-    count_groups<float, NI>(a, key, g32);
-    close = keep_groups<float>(a, g32, groups_by_score ? 4.f * slack : 0.f, bits);   // (each of two sums of two)
-    if (!by_score) {
-#pragma unroll
-      for (int i = 0; i < NI; i++) key[i] = by_logit(l[i]);
-    }
-    drop_groups<float, NI>(a, bits, key);
-  }
-  if (!close) win = pick<T, float, NI>(a, row, key, l, bias, by_score ? 2.f * slack : 0.f, close);
-  if (close) {
-    double z = 1., q[NI];
-    if (a.scoring == 0) {
-      double s = 0.;
-#pragma unroll
-      for (int i = 0; i < NI; i++) s += l[i] == -INFINITY ? 0. : exp((double)l[i] - (double)fm);
-      z = rt_sum(s);
-    }
-#pragma unroll
-    for (int i = 0; i < NI; i++) {
-      const double v = (a.scoring == 0 ? exp((double)l[i] - (double)fm) / z : 1. / (1. + exp(-(double)l[i]))) + (double)bias[i];
-      q[i] = l[i] == -INFINITY ? -INFINITY : v == v ? v : INFINITY;
-    }
-    if (a.G > 1) {
-      __syncwarp();   // (the floats' sums have been read)
-      count_groups<double, NI>(a, q, grp);
-      keep_groups<double>(a, grp, 0., bits);
-      if (!by_score) {
-#pragma unroll
-        for (int i = 0; i < NI; i++) q[i] = by_logit(l[i]);
-      }
-      drop_groups<double, NI>(a, bits, q);
-    }
-    win = pick<T, double, NI>(a, row, q, l, bias, 0., close);
-  }
+  fz = rt_sum(z);
+}
+
+// lane r has the r-th pick, or -1
+template <typename T>
+__device__ __forceinline__ void store_picks(const RouteArgs& a, int token, const T* row, int win, float fm, float fz) {
+  const int lane = threadIdx.x & 31;
   float score = 0.f;
   if (win >= 0) {
     const float x = static_cast<float>(row[win]);
@@ -319,6 +239,242 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
     a.indices[at] = win;
     a.weights[at] = a.scale * score;
   }
+}
+
+// A token as 64 bits have it.
+template <typename T, int NI>
+__device__ __forceinline__ void route_exactly(const RouteArgs& a, int token, const T* row, double* grp, uint32_t* bits) {
+  const int e0 = NI * (threadIdx.x & 31);
+  float fm = 0.f, fz = 1.f;
+  float l[NI];
+  double z = 1., q[NI];
+  load_row<T, NI>(row, a.E, a.whole, l);
+  if (a.scoring == 0) {
+    float e[NI];
+    softmax<NI>(l, e, fm, fz);
+    double s = 0.;
+#pragma unroll
+    for (int i = 0; i < NI; i++) s += l[i] == -INFINITY ? 0. : exp((double)l[i] - (double)fm);
+    z = rt_sum(s);
+  }
+#pragma unroll
+  for (int i = 0; i < NI; i++) {
+    double v = a.scoring == 0 ? exp((double)l[i] - (double)fm) / z : 1. / (1. + exp(-(double)l[i]));
+    if (a.bias != nullptr && e0 + i < a.E) v += (double)a.bias[e0 + i];
+    q[i] = l[i] == -INFINITY ? -INFINITY : v == v ? v : INFINITY;
+  }
+  if (a.G > 1) {
+    if (a.bias == nullptr && a.group_top == 1) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) q[i] = rt_first(l[i]);
+    }
+    __syncwarp();
+    count_groups<double, NI>(a, q, grp);
+    keep_groups<double>(a, grp, 0., bits);
+  }
+  if (a.bias == nullptr) {
+#pragma unroll
+    for (int i = 0; i < NI; i++) q[i] = rt_first(l[i]);
+  }
+  if (a.G > 1) drop_groups<double, NI>(a, bits, q);
+  store_picks<T>(a, token, row, pick<NI>(a, q), fm, fz);
+  __syncwarp();
+}
+
+__device__ __forceinline__ void sort_pair(uint32_t& a, uint32_t& b) {
+  const uint32_t m = max(a, b);
+  b = min(a, b);
+  a = m;
+}
+// descending, by a network of odd and even merges
+template <int N>
+__device__ __forceinline__ void sort_codes(uint32_t (&c)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+    for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; i++)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) sort_pair(c[i + j], c[i + j + k]);
+}
+
+__device__ __forceinline__ float fast_sigmoid(float x) {
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(x * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(s) : "f"(1.f + e));
+  return s;
+}
+// the two largest of (b0, b1) and (c0, c1), both in order
+__device__ __forceinline__ void merge_two(uint32_t c0, uint32_t c1, uint32_t& b0, uint32_t& b1) {
+  b1 = max(min(b0, c0), max(b1, c1));
+  b0 = max(b0, c0);
+}
+
+template <int NI>
+constexpr int route_ctas() { return NI <= 4 ? 10 : NI == 8 ? 8 : NI == 16 ? 4 : 2; }   // of an SM
+
+template <typename T, int NI>
+__global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kernel(const RouteArgs a) {
+  constexpr int IB = NI == 2 ? 6 : NI == 4 ? 7 : NI == 8 ? 8 : NI == 16 ? 9 : 10;   // bits of an expert's index
+  constexpr uint32_t IM = (1u << IB) - 1;
+  constexpr float UNITS = (float)(1ull << (32 - IB)) - 1024.f;
+  extern __shared__ double route_smem[];   // per warp, with groups: what they count, E keys, bits
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = NI * lane;
+  double* grp = route_smem + (size_t)warp * (a.G + a.E + 16);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(grp + a.G + a.E);
+  // what experts are ranked by, and groups; a logit of 16 bits is all in its code
+  const bool by_score = a.bias != nullptr, groups_by_score = by_score || a.group_top > 1;
+  const bool sure = !by_score && sizeof(T) == 2;
+  float bias[NI], lo = 0.f, hi = 1.f, slack = kRouteSlack;
+  bool odd = false;        // biases that a code cannot hold
+  if (by_score) {
+    load_row<float, NI>(a.bias, a.E, a.whole_bias, bias);
+    float least = INFINITY, most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+      if (e0 + i < a.E) {
+        odd |= !(fabsf(bias[i]) < 1e30f);
+        least = fminf(least, bias[i]);
+        most = fmaxf(most, bias[i]);
+      }
+    lo = -rt_max(-least);
+    hi = rt_max(most) + 1.f;
+    slack *= 1.f + fmaxf(fabsf(lo), fabsf(hi));
+    odd = __any_sync(kAll, odd);
+  }
+  // score + bias as fixed point: unit * s + shift, from 0 at the least bias
+  const float unit = UNITS / (hi - lo);
+  float shift[NI];
+#pragma unroll
+  for (int i = 0; i < NI; i++) shift[i] = by_score ? (bias[i] - lo) * unit : 0.f;
+  const uint32_t unsure = (uint32_t)fminf(2.f * slack * unit + 4.f, 1e9f);   // of two codes
+  const uint32_t close_by = by_score ? unsure : 0u, groups_close_by = groups_by_score ? 2 * unsure : 0u;
+  const int lanes = a.G > 1 ? a.size / NI : 1;   // of a group
+  const bool whole_groups = a.G > 1 && a.G <= 32 && a.size % NI == 0 && 32 % lanes == 0;
+
+  // Up to 32 tokens at a time, then those of them that 64 bits have to rank: the registers are free by then.
+  const int stride = gridDim.x * kRouteWarps;
+  int first = blockIdx.x * kRouteWarps + warp, it = 0;
+  uint32_t again = 0;
+  auto exactly = [&]() {
+    for (; again != 0; again &= again - 1) {
+      const int t = first + (__ffs(again) - 1) * stride;
+      route_exactly<T, NI>(a, t, static_cast<const T*>(a.logits) + (long long)t * a.E, grp, bits);
+    }
+  };
+  for (int token = first; token < a.T; token += stride, it++) {
+    if (it == 32) {
+      exactly();
+      first = token;
+      it = 0;
+    }
+    const T* row = static_cast<const T*>(a.logits) + (long long)token * a.E;
+    float l[NI], s[NI];
+    load_row<T, NI>(row, a.E, a.whole, l);
+    bool close = odd;
+    float fm = 0.f, fz = 1.f;
+    if (a.scoring == 0) {
+      softmax<NI>(l, s, fm, fz);
+      const float over = 1.f / fz;
+#pragma unroll
+      for (int i = 0; i < NI; i++) s[i] *= over;
+    } else if (by_score || (a.G > 1 && groups_by_score)) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) s[i] = fast_sigmoid(l[i]);
+    }
+    // a NaN's code would not come first; scores that are not numbers 64 bits have to deal with
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < NI; i++) nan |= l[i] != l[i];
+    nan |= fz != fz;
+    close |= __any_sync(kAll, nan);
+    uint32_t code[NI], by[NI];   // of the scores, and what experts are ranked by
+    if (by_score || (a.G > 1 && groups_by_score)) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const uint32_t v = (uint32_t)fmaf(s[i], unit, shift[i]);
+        code[i] = l[i] == -INFINITY ? 0u : (v << IB) + ((1u << IB) + IM - (uint32_t)(e0 + i));
+      }
+    }
+    if (!by_score) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) by[i] = l[i] == -INFINITY ? 0u : (rt_order(l[i] + 0.f) & ~IM) | (IM - (uint32_t)(e0 + i));
+    }
+    if (a.G > 1) {
+      if (whole_groups) {
+        uint32_t b0 = 0, b1 = 0;
+#pragma unroll
+        for (int i = 0; i < NI; i++) merge_two(groups_by_score ? code[i] : by[i], 0, b0, b1);
+        for (int o = 1; o < lanes; o <<= 1) merge_two(__shfl_xor_sync(kAll, b0, o), __shfl_xor_sync(kAll, b1, o), b0, b1);
+        // lane g comes to have group g: what it counts, and its index counted down; none without an expert
+        const uint32_t count = __shfl_sync(kAll, a.group_top > 1 ? (b0 >> IB) + (b1 >> IB) : b0 >> IB, lane * lanes & 31);
+        uint32_t mine = lane < a.G && count != 0 ? count << 5 | (31 - lane) : 0u, last = 0;
+        bool stays = false;
+        for (int r = 0; r < a.top_groups; r++) {
+          last = __reduce_max_sync(kAll, mine);
+          if (mine == last) {
+            mine = 0;
+            stays = true;
+          }
+        }
+        const uint32_t next = __reduce_max_sync(kAll, mine), kept = __ballot_sync(kAll, stays);
+        if (next != 0 && (sizeof(T) == 4 || groups_by_score)) close |= (last >> 5) - (next >> 5) <= groups_close_by;
+        if (!(kept >> (lane / lanes) & 1)) {
+#pragma unroll
+          for (int i = 0; i < NI; i++) code[i] = by[i] = 0;
+        }
+      } else {
+        float* g32 = reinterpret_cast<float*>(grp);
+        float key[NI];
+#pragma unroll
+        for (int i = 0; i < NI; i++) key[i] = l[i] == -INFINITY ? -INFINITY : !groups_by_score ? l[i] : by_score ? s[i] + bias[i] : s[i];
+        __syncwarp();
+        count_groups<float, NI>(a, key, g32);
+        close |= keep_groups<float>(a, g32, groups_by_score ? 4.f * slack : 0.f, bits);
+#pragma unroll
+        for (int i = 0; i < NI; i++) key[i] = 0.f;
+        drop_groups<float, NI>(a, bits, key);
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+          if (key[i] < 0.f) code[i] = by[i] = 0;
+      }
+    }
+    if (by_score) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) by[i] = code[i];
+    }
+    sort_codes<NI>(by);
+    uint32_t mine = 0;       // lane r: the r-th pick's code; one more, where it has to be told how near that comes
+    const int rounds = a.top_k < 32 && !sure ? a.top_k + 1 : a.top_k;
+    for (int r = 0; r < rounds; r++) {
+      const uint32_t top = __reduce_max_sync(kAll, by[0]);
+      if (lane == r) mine = top;
+      if (by[0] == top) {
+#pragma unroll
+        for (int i = 0; i < NI - 1; i++) by[i] = by[i + 1];
+        by[NI - 1] = 0;
+      }
+    }
+    if (!sure) {
+      const uint32_t before = __shfl_up_sync(kAll, mine, 1);
+      const bool near = lane > 0 && mine != 0 && (before >> IB) - (mine >> IB) <= close_by;
+      if (__any_sync(kAll, near)) {
+        // equals in every bit keep the order of their indices; what follows the last one is not known
+        bool same = false;
+        if (near && lane < a.top_k) {
+          const int e = (int)(IM - (mine & IM)), f = (int)(IM - (before & IM));
+          same = static_cast<float>(row[e]) == static_cast<float>(row[f]) && (!by_score || a.bias[e] == a.bias[f]);
+        }
+        close |= __any_sync(kAll, near && !same);
+      }
+      close |= a.top_k == 32;
+    }
+    if (close) again |= 1u << it;
+    else store_picks<T>(a, token, row, lane < a.top_k && mine != 0 ? (int)(IM - (mine & IM)) : -1, fm, fz);
+  }
+  exactly();
 }
 
 // dl from dw. A warp per token; everything but the picks is zero, except with softmax scores that are not renormalised.
@@ -401,13 +557,20 @@ cudaError_t route_launch(RouteArgs& a, cudaStream_t st) {
     route_backward_kernel<T, NI><<<grid, 32 * kRouteWarps, 0, st>>>(a);
     return cudaGetLastError();
   }
+  a.whole_bias = a.E % NI == 0 && (reinterpret_cast<uintptr_t>(a.bias) | (uintptr_t)(a.E * 4)) % (NI == 2 ? 8 : 16) == 0;
   a.size = a.E / a.G;
+  // as many CTAs as the GPU holds at once: more would wait for the first to be through with all their tokens
+  int dev = 0, sms = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (err != cudaSuccess) return err;
+  const unsigned room = (unsigned)(route_ctas<NI>() * sms);
   const size_t smem = a.G > 1 ? (size_t)kRouteWarps * (a.E + a.G + 16) * sizeof(double) : 0;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(route_kernel<T, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  route_kernel<T, NI><<<grid, 32 * kRouteWarps, smem, st>>>(a);
+  route_kernel<T, NI><<<grid < room ? grid : room, 32 * kRouteWarps, smem, st>>>(a);
   return cudaGetLastError();
 }
 template <typename T>

@@ -14,7 +14,7 @@ struct RouteArgs {
   float* weights;      // [T, top_k]
   const float* dw;     // [T, top_k]  (gradient only)
   void* dlogits;       // [T, E], or nullptr: the forward pass
-  int size, whole;     // set by the launch: experts of a group; a lane's experts are read at once
+  int size, whole, whole_bias;  // set by the launch: experts of a group; a lane's logits, biases are read at once
 };
 cudaError_t launch_route(RouteArgs a, cudaStream_t st);
 
