@@ -129,12 +129,17 @@ _front = None  # the module, or False where there is none that can be used
 
 
 def torch_front():
-    """The native front of quantized_matmul (csrc/kq_torch.cpp), or None where it was not built, or not for this torch: the
+    """The native front of quantized_matmul, lora_update and moe_router_grouped (csrc/kq_torch.cpp), or None where it was not built, or not for this torch: the
     library itself does not know torch, and every product works without the front, through ctypes."""
     global _front
     if _front is None:
         _front = _load_front(HERE / "_kq_torch.so") or False
     return _front or None
+
+
+def _warn_unused(path, why):
+    warnings.warn(f"mlx_kquant_b200: {path.name} is not used ({why}); build it again with make -C {HERE / 'csrc'}. "
+                  "Products of a few rows take some microseconds more of host time without it.", RuntimeWarning, stacklevel=5)
 
 
 def _load_front(path):
@@ -152,12 +157,16 @@ def _load_front(path):
         if built_for != torch.__version__:
             raise ImportError(f"built for torch {built_for}, this is {torch.__version__}")
     except (ImportError, OSError) as e:
-        warnings.warn(f"mlx_kquant_b200: {path.name} is not used ({e}); build it again with make -C {HERE / 'csrc'}. "
-                      "Products of a few rows take some microseconds more of host time without it.", RuntimeWarning, stacklevel=4)
+        _warn_unused(path, e)
         return None
     handle = lib()
-    module.init(*[C.cast(getattr(handle, name), C.c_void_p).value for name in
-                  ("kq_codec_find", "kq_codec_info", "kq_quantized_matmul_workspace_bytes", "kq_quantized_matmul")])
+    try:
+        module.init(*[C.cast(getattr(handle, name), C.c_void_p).value for name in
+                      ("kq_codec_find", "kq_codec_info", "kq_quantized_matmul_workspace_bytes", "kq_quantized_matmul",
+                       "kq_lora_update", "kq_lora_plan_bytes", "kq_lora_plan", "kq_moe_router_grouped")])
+    except TypeError:   # built from an older source, for the same torch
+        _warn_unused(path, "built for another version of this package")
+        return None
     return module
 
 

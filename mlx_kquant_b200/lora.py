@@ -92,6 +92,25 @@ class _Call:
         return dx, da, db
 
 
+def _first_lora(*args):
+    """The first call of _front_lora: the native front takes its place, or a stand-in where there is none."""
+    global _front_lora
+    front = _lib.torch_front()
+    _front_lora = front.lora if front is not None else lambda *args: None
+    return _front_lora(*args)
+
+
+_front_lora = _first_lora
+
+
+def front_update(y, x, a, b, adapter_ids, scaling, indices):
+    """The usual call without gradients, in one native call, or None: not for that path."""
+    out = _front_lora(y, x, a, b, adapter_ids, scaling, indices, DIRECT_ROWS)
+    if type(out) is int:
+        check(out)
+    return out
+
+
 class _Update(torch.autograd.Function):
     @staticmethod
     def forward(ctx, call, y, x, a, b):
@@ -177,6 +196,10 @@ def lora_update(y, x, a, b, adapter_ids=None, scaling=None, *, out=None, stream=
     Returns a tensor like y, or writes to `out`, which may be y. Differentiable in y, x, a and b (not with `out` or `stream`). The
     same call gives the same bits. A training step can be captured into a CUDA graph; as for every operator of torch, no eager
     autograd graph of the same leaves may be alive then."""
+    if out is None and stream is None:
+        done = front_update(y, x, a, b, adapter_ids, scaling, None)
+        if done is not None:
+            return done
     op = "lora_update"
     if a.dim() == 2 and b.dim() == 2:
         a, b = a.unsqueeze(0), b.unsqueeze(0)

@@ -891,6 +891,17 @@ def _route_grouped(logits, top_k, n_groups, top_groups, scoring, bias, group_top
     return idx, w
 
 
+def _first_route(*args):
+    """The first call of _front_route: the native front takes its place, or a stand-in where there is none."""
+    global _front_route
+    front = _lib.torch_front()
+    _front_route = front.route if front is not None else lambda *args: None
+    return _front_route(*args)
+
+
+_front_route = _first_route
+
+
 def moe_router_grouped(logits, top_k, n_groups=1, top_groups=1, *, scoring="sigmoid", bias=None, group_top=2,
                        norm_topk_prob=True, scale=1.0):
     """Routing to experts in groups, with a bias for balance: score the E columns of logits [T, E] ("sigmoid" or "softmax", in
@@ -905,6 +916,11 @@ def moe_router_grouped(logits, top_k, n_groups=1, top_groups=1, *, scoring="sigm
     Returns (indices [T, top_k] int32, weights [T, top_k] float32), the index type and the weights that `moe_glu` and the fused ops
     take; the weights are differentiable in the logits (CUDA tensors: one kernel each way; host tensors: torch ops).
     E <= 1024, top_k <= 32."""
+    done = _front_route(logits, top_k, n_groups, top_groups, scoring, bias, group_top, norm_topk_prob, scale)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done)
+        return done
     op = "moe_router_grouped"
     if scoring not in ("sigmoid", "softmax"):
         raise ValueError(f"[mlx_kquant.{op}] unknown scoring '{scoring}'.")
@@ -939,8 +955,12 @@ def gather_lora_update(y, x, a, b, indices, adapter_ids=None, scaling=None, *, o
     [T, R, K], one per slot; a [G, E, r, K] and b [G, E, N, r] (without the first axis: one adapter for all); indices [T, R];
     adapter_ids [T], None: adapter 0. A slot whose expert is outside [0, E) or whose adapter is outside [0, G) stays y's. The rest is
     as in `lora_update`."""
-    from .lora import _Call, _i32, _update
+    from .lora import _Call, _i32, _update, front_update
 
+    if out is None and stream is None and isinstance(indices, torch.Tensor):
+        done = front_update(y, x, a, b, adapter_ids, scaling, indices)
+        if done is not None:
+            return done
     op = "gather_lora_update"
     if a.dim() == 3 and b.dim() == 3:
         a, b = a.unsqueeze(0), b.unsqueeze(0)
