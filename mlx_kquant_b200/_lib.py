@@ -163,7 +163,9 @@ def _load_front(path):
     try:
         module.init(*[C.cast(getattr(handle, name), C.c_void_p).value for name in
                       ("kq_codec_find", "kq_codec_info", "kq_quantized_matmul_workspace_bytes", "kq_quantized_matmul",
-                       "kq_lora_update", "kq_lora_plan_bytes", "kq_lora_plan", "kq_moe_router_grouped")])
+                       "kq_lora_update", "kq_lora_plan_bytes", "kq_lora_plan", "kq_lora_saved_bytes",
+                       "kq_lora_backward_workspace_bytes", "kq_lora_backward", "kq_moe_router_grouped",
+                       "kq_moe_router_grouped_backward", "kq_last_error")])
     except TypeError:   # built from an older source, for the same torch
         _warn_unused(path, "built for another version of this package")
         return None

@@ -1,5 +1,5 @@
 // quantized_matmul of a few rows, the low-rank updates and the grouped router, from Python objects to the launch in one native call.
-// (The latter two without gradients: one token's update took the host 26 us in Python, its routing 13.) The Python form of the same steps
+// (One token's update took the host 26 us in Python, its routing 13, the routing and its gradient 97.) The Python form of the same steps
 // (ops.py) took 9 of the 14 us that a one-row product costs the host: attribute lookups, shape tuples, a ctypes call of
 // sixteen arguments. It stays for every other form: this one answers None to whatever it does not know - subclasses of
 // Tensor, tensors without storage of their own (vmap, tracing), CPU tensors, another device than the current one, operands
@@ -8,8 +8,12 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <cstring>
 
 #include "../../include/kquant_b200.h"
 
@@ -23,11 +27,17 @@ decltype(&kq_quantized_matmul) matmul;
 decltype(&kq_lora_update) lora_update;
 decltype(&kq_lora_plan_bytes) lora_plan_bytes;
 decltype(&kq_lora_plan) lora_plan;
+decltype(&kq_lora_saved_bytes) lora_saved_bytes;
+decltype(&kq_lora_backward_workspace_bytes) lora_backward_workspace_bytes;
+decltype(&kq_lora_backward) lora_backward;
 decltype(&kq_moe_router_grouped) router_grouped;
+decltype(&kq_moe_router_grouped_backward) router_grouped_backward;
+decltype(&kq_last_error) last_error;
 
 PyObject* init(PyObject*, PyObject* args) {
-  unsigned long long p[8];
-  if (!PyArg_ParseTuple(args, "KKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7])) return nullptr;
+  unsigned long long p[13];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8], &p[9], &p[10], &p[11], &p[12]))
+    return nullptr;
   codec_find = reinterpret_cast<decltype(codec_find)>(p[0]);
   codec_info = reinterpret_cast<decltype(codec_info)>(p[1]);
   workspace_bytes = reinterpret_cast<decltype(workspace_bytes)>(p[2]);
@@ -35,7 +45,12 @@ PyObject* init(PyObject*, PyObject* args) {
   lora_update = reinterpret_cast<decltype(lora_update)>(p[4]);
   lora_plan_bytes = reinterpret_cast<decltype(lora_plan_bytes)>(p[5]);
   lora_plan = reinterpret_cast<decltype(lora_plan)>(p[6]);
-  router_grouped = reinterpret_cast<decltype(router_grouped)>(p[7]);
+  lora_saved_bytes = reinterpret_cast<decltype(lora_saved_bytes)>(p[7]);
+  lora_backward_workspace_bytes = reinterpret_cast<decltype(lora_backward_workspace_bytes)>(p[8]);
+  lora_backward = reinterpret_cast<decltype(lora_backward)>(p[9]);
+  router_grouped = reinterpret_cast<decltype(router_grouped)>(p[10]);
+  router_grouped_backward = reinterpret_cast<decltype(router_grouped_backward)>(p[11]);
+  last_error = reinterpret_cast<decltype(last_error)>(p[12]);
   Py_RETURN_NONE;
 }
 
@@ -101,15 +116,135 @@ PyObject* qmm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// a plain, dense tensor on the current device that no gradient is wanted of
-bool ready(const at::Tensor& t) {
-  return plain(t) && t.is_contiguous() && t.device().index() == c10::cuda::current_device() &&
-         !(t.requires_grad() && c10::GradMode::is_enabled());
-}
+// a plain, dense tensor on the current device
+bool ready(const at::Tensor& t) { return plain(t) && t.is_contiguous() && t.device().index() == c10::cuda::current_device(); }
+
+bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
 
 int type_of(const at::Tensor& t) {
   return t.scalar_type() == at::kFloat ? KQ_F32 : t.scalar_type() == at::kHalf ? KQ_F16 : t.scalar_type() == at::kBFloat16 ? KQ_BF16 : -1;
 }
+
+at::Tensor bytes_of(size_t n, const at::Tensor& like) {
+  return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false));
+}
+void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// a low-rank update, checked
+struct Lora {
+  int type, param, K, N, rank, G, E, slots;
+  int64_t rows;
+  bool shared;
+  at::Tensor ids, experts, scaling;   // undefined: none
+  float scale;
+
+  const int32_t* id() const { return static_cast<const int32_t*>(data(ids)); }
+  const uint32_t* expert() const { return static_cast<const uint32_t*>(data(experts)); }
+  const float* factor() const { return static_cast<const float*>(data(scaling)); }
+  bool grouped() const { return ids.defined() || experts.defined(); }
+
+  at::Tensor plan(const at::Tensor& like) const { return grouped() ? bytes_of(lora_plan_bytes(rows, G * E), like) : at::Tensor(); }
+  int order(const at::Tensor& plan, cudaStream_t stream) const {
+    return plan.defined() ? lora_plan(id(), expert(), rows, slots, G, E, plan.data_ptr(), plan.numel(), stream) : 0;
+  }
+  int update(const at::Tensor& y, const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const at::Tensor& out, const at::Tensor& saved,
+             const at::Tensor& plan, cudaStream_t stream) const {
+    return lora_update(x.data_ptr(), type, rows, K, K, slots, shared, a.data_ptr(), b.data_ptr(), param, rank, N, G, E, id(), expert(), factor(),
+                       scale, y.data_ptr(), N, out.data_ptr(), N, data(saved), data(plan), plan.defined() ? plan.numel() : 0, stream);
+  }
+};
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void once(const char* op) {
+  TORCH_CHECK(!c10::GradMode::is_enabled(), "[mlx_kquant.", op, "] has a gradient, but that has none of its own (create_graph).");
+}
+
+struct LoraFunction : torch::autograd::Function<LoraFunction> {
+  // (the call's own tensors have no gradient: they go in and out by value)
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const Lora& call) {
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+    at::Tensor out = at::empty(y.sizes(), y.options().requires_grad(false)), plan = call.plan(y);
+    at::Tensor saved = bytes_of(lora_saved_bytes(call.rows, call.rank, call.param), y);
+    int rc = call.order(plan, stream);
+    if (rc == 0) rc = call.update(y, x, a, b, out, saved, plan, stream);
+    TORCH_CHECK(rc == 0, last_error());
+    ctx->save_for_backward({x, a, b, saved, plan, call.ids, call.experts, call.scaling});
+    ctx->saved_data["call"] = std::vector<int64_t>{call.type, call.param, call.K, call.N, call.rank, call.G, call.E, call.slots, call.rows, call.shared};
+    ctx->saved_data["scale"] = (double)call.scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("lora_update");
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    const auto kept = ctx->get_saved_variables();
+    const auto v = ctx->saved_data["call"].toIntVector();
+    const at::Tensor &x = kept[0], &a = kept[1], &b = kept[2], &saved = kept[3], &plan = kept[4], dy = grads[0].contiguous();
+    const Lora call{(int)v[0], (int)v[1], (int)v[2], (int)v[3], (int)v[4], (int)v[5], (int)v[6], (int)v[7], v[8], v[9] != 0,
+                    kept[5], kept[6], kept[7], (float)ctx->saved_data["scale"].toDouble()};
+    if (ctx->needs_input_grad(0)) out[0] = grads[0];
+    const c10::cuda::CUDAGuard on(x.device());
+    if (ctx->needs_input_grad(1)) out[1] = at::empty_like(x);
+    if (ctx->needs_input_grad(2)) out[2] = at::empty_like(a);
+    if (ctx->needs_input_grad(3)) out[3] = at::empty_like(b);
+    if (!out[1].defined() && !out[2].defined() && !out[3].defined()) return out;
+    const at::Tensor ws = bytes_of(std::max<size_t>(256, lora_backward_workspace_bytes(call.rows, call.slots, call.shared, call.K, call.rank, call.param)), x);
+    const int rc = lora_backward(dy.data_ptr(), call.type, call.rows, call.N, call.N, x.data_ptr(), call.K, call.K, call.slots, call.shared, a.data_ptr(),
+                                 b.data_ptr(), call.param, call.rank, call.G, call.E, call.id(), call.expert(), call.factor(), call.scale, saved.data_ptr(),
+                                 data(out[1]), data(out[2]), data(out[3]), data(plan), plan.defined() ? plan.numel() : 0, ws.data_ptr(), ws.numel(),
+                                 c10::cuda::getCurrentCUDAStream(x.device().index()).stream());
+    TORCH_CHECK(rc == 0, last_error());
+    return out;
+  }
+};
+
+struct Route {
+  int type, top_k, groups, top_groups, group_top, norm;
+  std::string scoring;
+  const float* bias;
+  float scale;
+  int run(const at::Tensor& logits, at::Tensor& idx, at::Tensor& w) const {
+    const int64_t T = logits.size(0);
+    idx = at::empty({T, top_k}, logits.options().dtype(at::kInt).requires_grad(false));
+    w = at::empty({T, top_k}, logits.options().dtype(at::kFloat).requires_grad(false));
+    return router_grouped(logits.data_ptr(), type, T, (int)logits.size(1), top_k, groups, top_groups, group_top, scoring.c_str(), bias, norm, scale,
+                          static_cast<int32_t*>(idx.data_ptr()), static_cast<float*>(w.data_ptr()),
+                          c10::cuda::getCurrentCUDAStream(logits.device().index()).stream());
+  }
+};
+
+struct RouteFunction : torch::autograd::Function<RouteFunction> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const Route& call) {
+    at::Tensor idx, w;
+    const int rc = call.run(logits, idx, w);
+    TORCH_CHECK(rc == 0, last_error());
+    ctx->mark_non_differentiable({idx});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, idx});
+    ctx->saved_data["call"] = std::vector<int64_t>{call.type, call.top_k, call.norm};
+    ctx->saved_data["scoring"] = call.scoring;
+    ctx->saved_data["scale"] = (double)call.scale;
+    return {idx, w};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("moe_router_grouped");
+    variable_list out(2);
+    if (!grads[1].defined()) return out;
+    const auto kept = ctx->get_saved_variables();
+    const auto v = ctx->saved_data["call"].toIntVector();
+    const at::Tensor &logits = kept[0], &idx = kept[1], dw = grads[1].contiguous();
+    const c10::cuda::CUDAGuard on(logits.device());
+    out[0] = at::empty_like(logits);
+    const int rc = router_grouped_backward(logits.data_ptr(), (int)v[0], logits.size(0), (int)logits.size(1), (int)v[1],
+                                           ctx->saved_data["scoring"].toStringRef().c_str(), (int)v[2], (float)ctx->saved_data["scale"].toDouble(),
+                                           static_cast<const int32_t*>(idx.data_ptr()), static_cast<const float*>(dw.data_ptr()), out[0].data_ptr(),
+                                           c10::cuda::getCurrentCUDAStream(logits.device().index()).stream());
+    TORCH_CHECK(rc == 0, last_error());
+    return out;
+  }
+};
 
 // lora(y, x, a, b, adapter_ids, scaling, indices, direct_rows) -> the updated rows, an error code of the library, or None: not for
 // this path. indices: None (a [adapters, r, K]), or the experts of the slots (a [adapters, experts, r, K]).
@@ -134,7 +269,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t rows = y.numel() / N;
   int64_t slots = 1;
   bool shared = false;
-  const void *ids = nullptr, *experts = nullptr;
+  at::Tensor ids, experts;
   if (gathered) {
     if (!THPVariable_CheckExact(args[6])) Py_RETURN_NONE;
     const at::Tensor& idx = THPVariable_Unpack(args[6]);
@@ -143,7 +278,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t n) {
     shared = x.dim() == 2;
     if (!(shared || x.dim() == 3) || x.size(0) != idx.size(0) || (!shared && x.size(1) != idx.size(1))) Py_RETURN_NONE;
     slots = idx.size(1);
-    experts = idx.data_ptr();
+    experts = idx;
   } else {
     if (x.dim() != y.dim()) Py_RETURN_NONE;
     for (int64_t i = 0; i + 1 < x.dim(); i++)
@@ -156,11 +291,11 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (int64_t i = 0; i < t.dim(); i++)
       if (t.size(i) != x.size(i)) Py_RETURN_NONE;
     if (!gathered) slots = rows / t.numel();
-    ids = t.data_ptr();
+    ids = t;
   } else if (G != 1) {
     Py_RETURN_NONE;
   }
-  const float* scaling = nullptr;
+  at::Tensor scaling;
   double scale = 1.;
   if (args[5] != Py_None) {
     if (PyFloat_CheckExact(args[5])) {
@@ -169,26 +304,23 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (!THPVariable_CheckExact(args[5])) Py_RETURN_NONE;
       const at::Tensor& t = THPVariable_Unpack(args[5]);
       if (!ready(t) || t.requires_grad() || t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != G) Py_RETURN_NONE;
-      scaling = t.data_ptr<float>();
+      scaling = t;
     }
   }
-  at::Tensor out = at::empty(y.sizes(), y.options().requires_grad(false)), plan;
-  size_t bytes = 0;
-  if (rows > PyLong_AsLongLong(args[7]) && (ids != nullptr || experts != nullptr)) {
-    bytes = lora_plan_bytes(rows, (int)(G * E));
-    plan = at::empty({(int64_t)bytes}, y.options().dtype(at::kByte).requires_grad(false));
-  }
+  const int64_t direct = PyLong_AsLongLong(args[7]);
   if (PyErr_Occurred()) return nullptr;
-  if (!plain(out) || (bytes != 0 && !plain(plan))) Py_RETURN_NONE;  // (under a dispatch mode)
+  if (rows > INT32_MAX - 64) Py_RETURN_NONE;
+  const Lora call{type, param, (int)K, (int)N, (int)r, (int)G, (int)E, (int)slots, rows, shared, ids, experts, scaling, (float)scale};
+  if (wants_gradient(y) || wants_gradient(x) || wants_gradient(a) || wants_gradient(b))
+    return THPVariable_Wrap(LoraFunction::apply(y, x, a, b, call));
+  at::Tensor out = at::empty(y.sizes(), y.options().requires_grad(false)), plan;
+  if (rows > direct) plan = call.plan(y);
+  if (!plain(out) || (plan.defined() && !plain(plan))) Py_RETURN_NONE;  // (under a dispatch mode)
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
-  int rc = 0;
+  int rc;
   Py_BEGIN_ALLOW_THREADS
-  if (bytes != 0)
-    rc = lora_plan(static_cast<const int32_t*>(ids), static_cast<const uint32_t*>(experts), rows, (int)slots, (int)G, (int)E, plan.data_ptr(), bytes, stream);
-  if (rc == 0)
-    rc = lora_update(x.data_ptr(), type, rows, (int)K, K, (int)slots, shared, a.data_ptr(), b.data_ptr(), param, (int)r, (int)N, (int)G, (int)E,
-                     static_cast<const int32_t*>(ids), static_cast<const uint32_t*>(experts), scaling, (float)scale, y.data_ptr(), N,
-                     out.data_ptr(), N, nullptr, bytes != 0 ? plan.data_ptr() : nullptr, bytes, stream);
+  rc = call.order(plan, stream);
+  if (rc == 0) rc = call.update(y, x, a, b, out, at::Tensor(), plan, stream);
   Py_END_ALLOW_THREADS
   if (rc != 0) return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(out));
@@ -211,7 +343,7 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t n) {
     v[i] = PyLong_AsLong(args[at_[i]]);
     if (PyErr_Occurred()) return nullptr;
   }
-  const int64_t T = logits.size(0), E = logits.size(1);
+  const int64_t E = logits.size(1);
   if (E < 1 || E > 1024 || v[0] < 1 || v[0] > 32) Py_RETURN_NONE;
   const float* bias = nullptr;
   if (args[5] != Py_None) {
@@ -225,16 +357,20 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (v[i] < 0 || v[i] > INT32_MAX) Py_RETURN_NONE;
   const char* scoring = PyUnicode_AsUTF8(args[4]);
   if (scoring == nullptr) return nullptr;
-  at::Tensor idx = at::empty({T, v[0]}, logits.options().dtype(at::kInt).requires_grad(false));
-  at::Tensor w = at::empty({T, v[0]}, logits.options().dtype(at::kFloat).requires_grad(false));
-  if (!plain(idx) || !plain(w)) Py_RETURN_NONE;
-  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(logits.device().index()).stream();
-  int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = router_grouped(logits.data_ptr(), type, T, (int)E, (int)v[0], (int)v[1], (int)v[2], (int)v[3], scoring, bias, args[7] == Py_True,
-                      (float)PyFloat_AS_DOUBLE(args[8]), idx.data_ptr<int32_t>(), w.data_ptr<float>(), stream);
-  Py_END_ALLOW_THREADS
-  if (rc != 0) return PyLong_FromLong(rc);
+  // (what the kernel refuses is refused here, by the Python form, before a graph is made)
+  if (v[0] > E || v[1] < 1 || E % v[1] != 0 || v[2] < 1 || v[2] > v[1] || v[3] < 1 || v[3] > 2 || v[2] * (E / v[1]) < v[0] ||
+      (std::strcmp(scoring, "sigmoid") != 0 && std::strcmp(scoring, "softmax") != 0))
+    Py_RETURN_NONE;
+  const Route call{type, (int)v[0], (int)v[1], (int)v[2], (int)v[3], args[7] == Py_True, scoring, bias, (float)PyFloat_AS_DOUBLE(args[8])};
+  at::Tensor idx, w;
+  if (wants_gradient(logits)) {
+    auto out = RouteFunction::apply(logits, call);
+    idx = out[0];
+    w = out[1];
+  } else {
+    const int rc = call.run(logits, idx, w);
+    if (rc != 0) return PyLong_FromLong(rc);
+  }
   PyObject *i = THPVariable_Wrap(std::move(idx)), *j = i != nullptr ? THPVariable_Wrap(std::move(w)) : nullptr;
   PyObject* both = j != nullptr ? PyTuple_Pack(2, i, j) : nullptr;
   Py_XDECREF(i);

@@ -82,3 +82,42 @@ def test_router(monkeypatch):
             assert q[0] is p[0], (p, q)          # refused by both, as one kind of error
         else:
             assert same(p, q), kw
+
+
+@pytest.mark.parametrize("T", [5, 200])
+def test_gradients(monkeypatch, T):
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    ids = torch.randint(-1, 4, (T,), device="cuda", generator=g, dtype=torch.int32)
+    idx = torch.randint(-1, 6, (T, 3), device="cuda", generator=g, dtype=torch.int32)
+    y, x, a, b = rnd(T, 40).bfloat16(), rnd(T, 64).bfloat16(), rnd(3, 8, 64) * 0.1, rnd(3, 40, 8) * 0.1
+    y3, a4, b4 = rnd(T, 3, 40).bfloat16(), rnd(3, 6, 8, 64) * 0.1, rnd(3, 6, 40, 8) * 0.1
+    logits, bias = rnd(T, 64), rnd(64) * 0.1
+
+    def step(op, leaves, want, *rest):
+        leaves = [t.detach().clone().requires_grad_(w) for t, w in zip(leaves, want)]
+        out = op(*leaves, *rest)
+        out = out[1] if isinstance(out, tuple) else out
+        assert out.requires_grad
+        dy = torch.ones(1, device="cuda", dtype=out.dtype).expand(out.shape)   # not contiguous
+        return (out.detach(), *torch.autograd.grad(out, [t for t in leaves if t.requires_grad], dy))
+
+    for want in ((1, 1, 1, 1), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 0, 0, 0)):
+        p, q = both(monkeypatch, lambda: step(kq.lora_update, (y, x, a, b), want, ids, None))
+        assert same(p, q), want
+        p, q = both(monkeypatch, lambda: step(moe.gather_lora_update, (y3, x, a4, b4), want, idx, ids, 0.5))
+        assert same(p, q), want
+    p, q = both(monkeypatch, lambda: step(lambda l: moe.moe_router_grouped(l, 4, 8, 3, bias=bias), (logits,), (1,)))
+    assert same(p, q)
+    # a second gradient is refused by both
+    for call in (lambda: step2(kq.lora_update, a, lambda t: (y, x, t, b, ids)), lambda: step2(moe.moe_router_grouped, logits, lambda t: (t, 4))):
+        for out in both(monkeypatch, call):
+            assert isinstance(out, tuple) and out[0] is RuntimeError, out
+
+
+def step2(op, leaf, args):
+    leaf = leaf.detach().clone().requires_grad_()
+    out = op(*args(leaf))
+    out = out[1] if isinstance(out, tuple) else out
+    first, = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)
+    return torch.autograd.grad(first.square().sum(), leaf)
