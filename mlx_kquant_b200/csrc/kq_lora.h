@@ -35,8 +35,9 @@ struct LoraPlan {
   int tile_rows;
 };
 struct LoraPlanLayout {
-  size_t order, offsets, tiles, total;
+  size_t order, offsets, tiles, counts, total;
   int n_tiles, tile_rows;
+  int chunk, chunks;   // entries of a CTA, and CTAs, where they are counted and placed in two launches; 0: in one
 };
 LoraPlanLayout lora_plan_layout(long long n, int n_groups);
 cudaError_t launch_lora_plan(const LoraGroups& g, void* plan, cudaStream_t st);

@@ -282,3 +282,38 @@ def test_offsets_beyond_32_bits():
     want = plain(y[::2], x[::2], a[-1:], b[-1:], np.zeros(2, int), [1.0])
     check(out[::2], want["y"])
     assert (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("n,slots,G,E", [(1, 1, 1, 1), (300, 3, 2, 5), (5000, 1, 3, 1), (4096, 8, 1, 128), (12288, 4, 2, 300), (33000, 8, 4, 60),
+                                         (200_000, 1, 40, 1), (140_000, 7, 1, 1023), (3000, 2, 1, 2000), (9000, 9, 900, 60)])
+def test_order_by_groups(n, slots, G, E):
+    """The plan: entries by group and stable, where each group starts, tiles that cover all of them once."""
+    from mlx_kquant_b200 import _lib
+    rng = np.random.default_rng(n)
+    ids = np.where(rng.random(n // slots) < 0.1, rng.choice([-1, G, 2 ** 31 - 1], n // slots), rng.integers(0, G, n // slots)).astype(np.int32)
+    ex = np.where(rng.random(n) < 0.1, -1, rng.integers(0, E + 1, n)).astype(np.int32)
+    L, NG = _lib.lib(), G * E
+    for use_ids, use_ex in ((True, True), (True, False), (False, True)):
+        if (not use_ids and G > 1) or (not use_ex and E > 1):
+            continue
+        plan = torch.full((L.kq_lora_plan_bytes(n, NG) + 256,), 0x5a, dtype=torch.uint8, device="cuda")
+        di, de = torch.from_numpy(ids).cuda(), torch.from_numpy(ex).cuda()
+        _lib.check(L.kq_lora_plan(di.data_ptr() if use_ids else None, de.data_ptr() if use_ex else None, n, slots, G, E, plan.data_ptr(),
+                                  plan.numel() - 256, torch.cuda.current_stream().cuda_stream))
+        got = plan.cpu().numpy()
+        assert (got[-256:] == 0x5a).all()
+        i, x = (np.repeat(ids, slots) if use_ids else np.zeros(n, int)), (ex if use_ex else np.zeros(n, int))
+        key = np.where((i >= 0) & (i < G) & (x >= 0) & (x < E), i.astype(np.int64) * E + x, NG)
+        up = lambda v: (v + 255) // 256 * 256  # noqa: E731
+        order = got[:4 * n].view(np.int32)
+        assert np.array_equal(order, np.argsort(key, kind="stable"))
+        offsets = got[up(4 * n):up(4 * n) + 4 * (NG + 2)].view(np.int32)
+        assert np.array_equal(offsets, np.concatenate([[0], np.cumsum(np.bincount(key, minlength=NG + 1))]))
+        height = 64 if n >= 24 * NG else 16
+        at = up(up(4 * n) + 4 * (NG + 2))
+        tiles = got[at:at + 16 * (n // height + NG + 1)].view(np.int32).reshape(-1, 4)
+        seen = np.zeros(n, int)
+        for g, start, rows, _ in tiles[tiles[:, 2] > 0]:
+            assert rows <= height and (key[order[start:start + rows]] == (g if g >= 0 else NG)).all()
+            seen[start:start + rows] += 1
+        assert (seen == 1).all()
