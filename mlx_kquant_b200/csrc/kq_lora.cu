@@ -210,18 +210,19 @@ __global__ void __launch_bounds__(kChunkThreads) plan_place_kernel(const LoraGro
 // asynchronous copies into a ring; both fragments are transposed on the way out of it (the contraction runs over the entries). Four
 // warps have 32 columns each, the other four the same columns and the other half of a stage's entries. fp16 rows are two bf16
 // terms, exactly. The CTAs of a cluster share a group's stages; all sums meet in a fixed order.
-template <typename PT, int RT>
+template <typename PT, int RT, bool SHORT>
 struct WgradShape {
   static constexpr int RP = 16 * RT, UN = sizeof(PT) == 4 ? 3 : 2, ROWS = 64, COLS = 128;
   static constexpr int IN = ROWS * COLS * 2, UV = ROWS * RP * 2, STAGE = IN + UN * UV;
-  static constexpr int STAGES = 96 * 1024 / STAGE > 5 ? 5 : 96 * 1024 / STAGE < 3 ? 3 : 96 * 1024 / STAGE;
+  // groups of one or two stages: fewer of them, more CTAs of an SM
+  static constexpr int STAGES = SHORT ? 2 : 96 * 1024 / STAGE > 5 ? 5 : 96 * 1024 / STAGE < 3 ? 3 : 96 * 1024 / STAGE;
   static constexpr int OUT = COLS * RP * 4;   // sums of a half of the warps, then of the CTA: in the ring's room
   static constexpr int RING = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
   static constexpr int SMEM = RING + (STAGES + 1) * ROWS * 4;   // and the entries of the stages
 };
-template <typename XT, typename PT, int RT, bool FAST>
+template <typename XT, typename PT, int RT, bool FAST, bool SHORT>
 __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) {
-  typedef WgradShape<PT, RT> S;
+  typedef WgradShape<PT, RT, SHORT> S;
   constexpr int XN = RowTerms<XT, bf16>::N, UN = S::UN, RP = S::RP;
   typedef Tile<S::COLS, 2> InTile;
   typedef Tile<RP, 2> UvTile;
@@ -380,10 +381,10 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
   if (C > 1) cluster.sync();
 }
 
-template <typename XT, typename PT, int RT, bool FAST>
+template <typename XT, typename PT, int RT, bool FAST, bool SHORT>
 cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
-  typedef WgradShape<PT, RT> S;
-  auto kern = wgrad_kernel<XT, PT, RT, FAST>;
+  typedef WgradShape<PT, RT, SHORT> S;
+  auto kern = wgrad_kernel<XT, PT, RT, FAST, SHORT>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -398,11 +399,15 @@ cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
+template <typename XT, typename PT, int RT, bool FAST>
+cudaError_t wgrad_length(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
+  return a.g.n <= 128LL * a.n_groups ? wgrad_launch<XT, PT, RT, FAST, true>(a, cluster, st) : wgrad_launch<XT, PT, RT, FAST, false>(a, cluster, st);
+}
 template <typename XT, typename PT, bool FAST>
 cudaError_t wgrad_rank(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
-  if (a.r <= 16) return wgrad_launch<XT, PT, 1, FAST>(a, cluster, st);
-  if (a.r <= 32) return wgrad_launch<XT, PT, 2, FAST>(a, cluster, st);
-  return wgrad_launch<XT, PT, 4, FAST>(a, cluster, st);
+  if (a.r <= 16) return wgrad_length<XT, PT, 1, FAST>(a, cluster, st);
+  if (a.r <= 32) return wgrad_length<XT, PT, 2, FAST>(a, cluster, st);
+  return wgrad_length<XT, PT, 4, FAST>(a, cluster, st);
 }
 template <typename XT, typename PT>
 cudaError_t wgrad_read(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
@@ -467,7 +472,10 @@ int set_rows(LoraArgs& a, const LoraCall& c, int& cluster) {
     mt = 16;
     a.n_clusters = (int)c.g.n;
   }
-  cluster = pick_cluster(std::min<long long>(a.n_clusters, c.g.n));
+  // tiles that have rows, as far as the host knows: those found one by one are no more than the groups; half of the groups' last
+  // tiles of a plan are counted (4072 entries of 128 groups: clusters of 1, 2, 4, 8 forward 47, 30, 37, 56 us)
+  const long long groups = (long long)c.g.G * c.g.E;
+  cluster = pick_cluster(a.direct ? std::min(c.g.n, groups) : grouped ? c.g.n / mt + std::min(c.g.n, groups) / 2 : a.n_clusters);
   return mt;
 }
 
@@ -596,7 +604,20 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
   a.u = v;
   a.shrink = 1;
   a.scale_u = 1;
-  if (dx != nullptr && !summed) {
+  const long long tokens = c.g.n / c.g.slots;
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(c.g.n, c.r, f32));
+  const int step = slot_columns(c.g.n, c.K);
+  // a token's slots share its row: their parts in float32, as many columns at a time as stay in L2, then the sum
+  auto columns = [&](int c0) {
+    a.c0 = c0;
+    a.c1 = std::min(c.K, c0 + step);
+    a.out = part;
+    a.out_f32 = 1;
+    a.out_stride = a.c1 - c0;
+  };
+  if (dx != nullptr && summed) {
+    columns(0);
+  } else if (dx != nullptr) {
     a.out = dx;
     a.out_stride = dx_stride;
   }
@@ -605,21 +626,14 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
     if ((e = tile_launch(c.types, a, true, mt, cluster, st)) != cudaSuccess) return e;
   }
   if (dx != nullptr && summed) {
-    const long long tokens = c.g.n / c.g.slots;
-    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(c.g.n, c.r, f32));
-    const int step = slot_columns(c.g.n, c.K);
-    a.shrink = 0;
-    a.out = part;
-    a.out_f32 = 1;
-    for (int c0 = 0; c0 < c.K; c0 += step) {
-      a.c0 = c0;
-      a.c1 = std::min(c.K, c0 + step);
-      a.out_stride = a.c1 - a.c0;
+    for (int c0 = 0;;) {
+      if ((e = launch_lora_sum_slots(part, c.g.slots, tokens, a.c1 - a.c0, static_cast<uint16_t*>(dx) + c0, dx_stride, f16 ? 1 : 2, st)) != cudaSuccess)
+        return e;
+      if ((c0 = a.c1) >= c.K) break;
+      a.shrink = 0;
+      columns(c0);
       set_reads(a, c, true);
       if ((e = tile_launch(c.types, a, true, mt, cluster, st)) != cudaSuccess) return e;
-      if ((e = launch_lora_sum_slots(part, c.g.slots, tokens, a.c1 - a.c0, static_cast<uint16_t*>(dx) + c0, dx_stride, f16 ? 1 : 2, st)) !=
-          cudaSuccess)
-        return e;
     }
   }
   LoraWgradArgs w{};
