@@ -216,12 +216,14 @@ struct WgradShape {
   static constexpr int IN = ROWS * COLS * 2, UV = ROWS * RP * 2, STAGE = IN + UN * UV;
   // groups of one or two stages: fewer of them, more CTAs of an SM
   static constexpr int STAGES = SHORT ? 2 : 96 * 1024 / STAGE > 5 ? 5 : 96 * 1024 / STAGE < 3 ? 3 : 96 * 1024 / STAGE;
-  static constexpr int OUT = COLS * RP * 4;   // sums of a half of the warps, then of the CTA: in the ring's room
+  // the CTA's sums, in the ring's room: [ranks][columns] or [columns][ranks], whichever the gradient is, in rows of these pitches
+  static constexpr int PITCH_R = COLS + 4, PITCH_C = RP + 8;
+  static constexpr int OUT = (RP * PITCH_R > COLS * PITCH_C ? RP * PITCH_R : COLS * PITCH_C) * 4;
   static constexpr int RING = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
   static constexpr int SMEM = RING + (STAGES + 1) * ROWS * 4;   // and the entries of the stages
 };
 template <typename XT, typename PT, int RT, bool FAST, bool SHORT>
-__global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) {
+__global__ void __launch_bounds__(kThreads, RT == 1 && SHORT ? 4 : RT <= 2 ? 2 : 1) wgrad_kernel(const LoraWgradArgs both) {
   typedef WgradShape<PT, RT, SHORT> S;
   constexpr int XN = RowTerms<XT, bf16>::N, UN = S::UN, RP = S::RP;
   typedef Tile<S::COLS, 2> InTile;
@@ -230,11 +232,15 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, q = lane & 3, cq = warp & 3, half = warp >> 2;
-  const int group = blockIdx.y, j0 = blockIdx.z * 64, c0 = blockIdx.x / C * S::COLS;
-  int start = 0, count = (int)a.g.n;
-  if (a.offsets != nullptr) {
-    start = a.offsets[group];
-    count = a.offsets[group + 1] - start;
+  // one launch for both gradients: the first's tiles, then the second's
+  const int tile = blockIdx.x / C;
+  const bool second = tile >= both.tiles;
+  const LoraWgrad a = both.of[second];
+  const int group = blockIdx.y, j0 = blockIdx.z * 64, c0 = (tile - (second ? both.tiles : 0)) * S::COLS;
+  int start = 0, count = (int)both.g.n;
+  if (both.offsets != nullptr) {
+    start = both.offsets[group];
+    count = both.offsets[group + 1] - start;
   }
   const int blocks = (count + S::ROWS - 1) / S::ROWS;
   const int b0 = (int)((long long)blocks * rank / C), nb = (int)((long long)blocks * (rank + 1) / C) - b0;
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
   int* s_entry = reinterpret_cast<int*>(smem + S::RING);
   auto entry_of = [&](int s) {
     const int t = (b0 + s) * S::ROWS + tid;
-    return tid >= S::ROWS || s >= nb || t >= count ? -1 : a.order != nullptr ? a.order[start + t] : t;
+    return tid >= S::ROWS || s >= nb || t >= count ? -1 : both.order != nullptr ? both.order[start + t] : t;
   };
   typedef Deal<S::ROWS, S::COLS, 2> InD;
   const uint32_t in_to = InTile::at(0, InD::row(), InD::chunk());
@@ -269,8 +275,8 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
 #pragma unroll
         for (int c = tid; c < S::ROWS * UvTile::CHUNKS; c += kThreads) {
           const int m = c / UvTile::CHUNKS, ch = c % UvTile::CHUNKS, e = entries[m];
-          const bool there = e >= 0 && j0 + 8 * ch < a.ru;
-          cp16(UvTile::at(at + S::IN + n * S::UV, m, ch), there ? a.uv + ((long long)n * a.g.n + e) * a.ru + j0 + 8 * ch : a.uv, there);
+          const bool there = e >= 0 && j0 + 8 * ch < both.ru;
+          cp16(UvTile::at(at + S::IN + n * S::UV, m, ch), there ? a.uv + ((long long)n * both.g.n + e) * both.ru + j0 + 8 * ch : a.uv, there);
         }
     }
     next++;
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
   }
   cp_wait<0>();
   __syncthreads();
-  // [columns][ranks] in shared memory: one half of the warps, then both; the CTAs of the cluster add and store a part of it each
+  // in shared memory as the gradient lies: one half of the warps, then both; the CTAs of the cluster add and store a part of it each
   float* s_out = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int turn = 1; turn >= 0; turn--) {
@@ -359,24 +365,57 @@ __global__ void __launch_bounds__(kThreads) wgrad_kernel(const LoraWgradArgs a) 
 #pragma unroll
         for (int n = 0; n < 2 * RT; n++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            float* o = s_out + (32 * cq + 16 * m + i + 8 * (k >> 1)) * RP + 8 * n + 2 * q + (k & 1);
-            *o = turn == 1 ? acc[m][n][k] : *o + acc[m][n][k];
+          for (int h = 0; h < 2; h++) {
+            const int c = 32 * cq + 16 * m + i + 8 * h, j = 8 * n + 2 * q;
+            float v0 = acc[m][n][2 * h], v1 = acc[m][n][2 * h + 1];
+            if (a.r_first) {
+              float *o = s_out + j * S::PITCH_R + c, *p = o + S::PITCH_R;
+              *o = turn == 1 ? v0 : *o + v0;
+              *p = turn == 1 ? v1 : *p + v1;
+            } else {
+              float2* o = reinterpret_cast<float2*>(s_out + c * S::PITCH_C + j);
+              if (turn == 0) {
+                v0 += o->x;
+                v1 += o->y;
+              }
+              *o = make_float2(v0, v1);
+            }
           }
     }
     __syncthreads();
   }
   if (C > 1) cluster.sync();
-  const float f = a.scaled ? factor_of(a.g, group) : 1.f;
-  const int r1 = min(RP, a.r - j0), cols = min(S::COLS, a.D - c0);
-  PT* out = static_cast<PT*>(a.out) + (long long)group * a.r * a.D;
-  for (int v = rank * kThreads + tid; v < cols * r1; v += C * kThreads) {
-    const int c = a.r_first ? v % cols : v / r1, j = a.r_first ? v / cols : v % r1;
-    float s = 0.f;
-    if (C == 1) s = s_out[c * RP + j];
-    else
-      for (int b = 0; b < C; b++) s += *cluster.map_shared_rank(s_out + c * RP + j, b);
-    out[a.r_first ? (long long)(j0 + j) * a.D + c0 + c : (long long)(c0 + c) * a.r + j0 + j] = PT(s * f);
+  const float f = a.scaled ? factor_of(both.g, group) : 1.f;
+  const int r1 = min(RP, both.r - j0), cols = min(S::COLS, a.D - c0);
+  PT* out = static_cast<PT*>(a.out) + (long long)group * both.r * a.D;
+  // rows of the gradient's tile: ranks (r_first) or columns; four neighbours a thread
+  const int length = a.r_first ? cols : r1, n_rows = a.r_first ? r1 : cols, pitch = a.r_first ? S::PITCH_R : S::PITCH_C;
+  const long long stride = a.r_first ? a.D : both.r;
+  out += a.r_first ? (long long)j0 * a.D + c0 : (long long)c0 * both.r + j0;
+  const int quads = a.r_first ? S::COLS / 4 : RP / 4;   // a power of two
+  const bool whole = length % 4 == 0 && stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(PT)) == 0;
+  const int at = 4 * (tid & (quads - 1));
+  for (int row = tid / quads + rank * (kThreads / quads); row < n_rows; row += C * (kThreads / quads)) {
+    if (at >= length) break;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < C; b++) {
+      const float4* p = reinterpret_cast<const float4*>(s_out + row * pitch + at);
+      const float4 v = C == 1 ? *p : *cluster.map_shared_rank(p, b);
+      s[0] += v.x;
+      s[1] += v.y;
+      s[2] += v.z;
+      s[3] += v.w;
+    }
+    PT* o = out + row * stride + at;
+    if (whole) {
+      alignas(16) PT v[4] = {PT(s[0] * f), PT(s[1] * f), PT(s[2] * f), PT(s[3] * f)};
+      if constexpr (sizeof(PT) == 4) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
+      else *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (at + k < length) o[k] = PT(s[k] * f);
+    }
   }
   if (C > 1) cluster.sync();
 }
@@ -388,7 +427,7 @@ cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.D + S::COLS - 1) / S::COLS * cluster), (unsigned)a.n_groups, (unsigned)((a.r + 63) / 64));
+  cfg.gridDim = dim3((unsigned)((a.tiles + (a.of[1].out != nullptr ? (a.of[1].D + S::COLS - 1) / S::COLS : 0)) * cluster), (unsigned)a.n_groups, (unsigned)((a.r + 63) / 64));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
@@ -411,7 +450,7 @@ cudaError_t wgrad_rank(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
 }
 template <typename XT, typename PT>
 cudaError_t wgrad_read(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
-  return a.by_in == kBy16 ? wgrad_rank<XT, PT, true>(a, cluster, st) : wgrad_rank<XT, PT, false>(a, cluster, st);
+  return a.of[0].by_in == kBy16 && (a.of[1].out == nullptr || a.of[1].by_in == kBy16) ? wgrad_rank<XT, PT, true>(a, cluster, st) : wgrad_rank<XT, PT, false>(a, cluster, st);
 }
 
 // ---------------------------------------------------------------------------------------------------- sum over slots
@@ -636,32 +675,26 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
       if ((e = tile_launch(c.types, a, true, mt, cluster, st)) != cudaSuccess) return e;
     }
   }
+  if (da == nullptr && db == nullptr) return cudaSuccess;
+  auto side = [&](const void* in, long long stride, int div, int D, const void* uv, int scaled, void* out, int r_first) {
+    return LoraWgrad{in, stride, div, D, static_cast<const uint16_t*>(uv), scaled, out, r_first, by(in, stride, D, 2)};
+  };
   LoraWgradArgs w{};
   w.g = c.g;
   w.r = c.r;
+  w.ru = a.ru;
   w.n_groups = c.g.G * c.g.E;
   w.order = a.plan.order;
   w.offsets = a.plan.offsets;
-  w.ru = a.ru;
+  int n = 0;
+  if (db != nullptr) w.of[n++] = side(dy, dy_stride, 1, c.N, u, 1, db, 0);
+  if (da != nullptr) w.of[n++] = side(c.x, c.x_stride, c.shared ? c.g.slots : 1, c.K, v, 0, da, 1);
+  w.tiles = (w.of[0].D + 127) / 128;
   // CTAs of a cluster share a group's stages of 64 entries, where the columns alone leave the GPU empty
-  const long long stages = (c.g.n / w.n_groups + 63) / 64;
-  auto wgrad = [&](const void* in, long long stride, int div, int D, const void* uv, int scaled, void* out, int r_first) {
-    w.in = in;
-    w.in_stride = stride;
-    w.in_div = div;
-    w.D = D;
-    w.uv = static_cast<const uint16_t*>(uv);
-    w.scaled = scaled;
-    w.out = out;
-    w.r_first = r_first;
-    w.by_in = by(in, stride, D, 2);
-    int cluster = pick_cluster((long long)w.n_groups * ((D + 127) / 128));
-    while (cluster > 1 && stages < 2 * cluster) cluster >>= 1;
-    return launch_lora_wgrad(w, f16 ? 1 : 2, f32, cluster, st);
-  };
-  if (db != nullptr && (e = wgrad(dy, dy_stride, 1, c.N, u, 1, db, 0)) != cudaSuccess) return e;
-  if (da != nullptr && (e = wgrad(c.x, c.x_stride, c.shared ? c.g.slots : 1, c.K, v, 0, da, 1)) != cudaSuccess) return e;
-  return cudaSuccess;
+  const long long stages = (c.g.n / w.n_groups + 63) / 64, all = w.tiles + (n > 1 ? (w.of[1].D + 127) / 128 : 0);
+  cluster = pick_cluster(w.n_groups * all);
+  while (cluster > 1 && stages < 2 * cluster) cluster >>= 1;
+  return launch_lora_wgrad(w, f16 ? 1 : 2, f32, cluster, st);
 }
 
 }  // namespace kq

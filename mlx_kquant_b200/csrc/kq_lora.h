@@ -71,20 +71,24 @@ cudaError_t launch_lora_tile_f16(const LoraArgs& a, bool backward, int mt, int c
 cudaError_t launch_lora_tile_bf16_f32(const LoraArgs& a, bool backward, int mt, int cluster, cudaStream_t st);
 cudaError_t launch_lora_tile_f16_f32(const LoraArgs& a, bool backward, int mt, int cluster, cudaStream_t st);
 
-// dw[g] = sum over the group's entries of in^T uv: [D, r] (rows_first 0) or [r, D] (1).
-struct LoraWgradArgs {
-  LoraGroups g;
+// dw[g] = sum over the group's entries of in^T uv: [D, r] (r_first 0) or [r, D] (1).
+struct LoraWgrad {
   const void* in;
   long long in_stride;
-  int in_div, D, r;
+  int in_div, D;
   const uint16_t* uv;    // [terms][n][ru]
-  int ru;
   int scaled;            // times the adapter's factor
-  void* out;
-  int r_first;           // out [groups, r, D], else [groups, D, r]
+  void* out;             // [groups, r, D] (r_first), else [groups, D, r]; nullptr: none
+  int r_first;
+  int by_in;
+};
+struct LoraWgradArgs {
+  LoraGroups g;
+  LoraWgrad of[2];             // one of them or both, in one launch
+  int tiles;                   // of 128 columns of the first
+  int r, ru;
   const int *order, *offsets;  // or nullptr: one group, rows in order
   int n_groups;
-  int by_in;
 };
 cudaError_t launch_lora_wgrad(const LoraWgradArgs& a, int in_dtype, int out_f32, int cluster, cudaStream_t st);
 
