@@ -454,13 +454,31 @@ cudaError_t wgrad_read(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------------- sum over slots
+// four neighbouring columns of a token a thread; part's rows are whole fours where `quads`
 template <typename XT>
-__global__ void __launch_bounds__(kThreads) sum_slots_kernel(const float* part, int slots, int cols, XT* out, long long out_stride) {
+__global__ void __launch_bounds__(kThreads) sum_slots_kernel(const float* part, int slots, int cols, XT* out, long long out_stride, bool quads) {
   const long long token = blockIdx.x;
-  for (int c = threadIdx.x; c < cols; c += kThreads) {
-    float s = 0.f;
-    for (int j = 0; j < slots; j++) s += part[(token * slots + j) * cols + c];
-    out[token * out_stride + c] = XT(s);
+  const int c = 4 * (blockIdx.y * kThreads + threadIdx.x);
+  if (c >= cols) return;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* p = part + token * slots * cols + c;
+  XT* o = out + token * out_stride + c;
+  if (quads) {
+#pragma unroll 8
+    for (int j = 0; j < slots; j++) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(p + (long long)j * cols));
+      s[0] += v.x;
+      s[1] += v.y;
+      s[2] += v.z;
+      s[3] += v.w;
+    }
+    const uint2 v = make_uint2(round_pair(s[0], s[1], XT()), round_pair(s[2], s[3], XT()));
+    *reinterpret_cast<uint2*>(o) = v;
+    return;
+  }
+  for (int k = 0; k < 4 && c + k < cols; k++) {
+    for (int j = 0; j < slots; j++) s[k] += p[(long long)j * cols + k];
+    o[k] = XT(s[k]);
   }
 }
 
@@ -582,8 +600,10 @@ cudaError_t launch_lora_wgrad(const LoraWgradArgs& a, int in_dtype, int out_f32,
 
 cudaError_t launch_lora_sum_slots(const float* part, int slots, long long tokens, int cols, void* out, long long out_stride, int dtype,
                                   cudaStream_t st) {
-  if (dtype == 1) sum_slots_kernel<__half><<<(unsigned)tokens, kThreads, 0, st>>>(part, slots, cols, static_cast<__half*>(out), out_stride);
-  else sum_slots_kernel<bf16><<<(unsigned)tokens, kThreads, 0, st>>>(part, slots, cols, static_cast<bf16*>(out), out_stride);
+  const dim3 grid((unsigned)tokens, (unsigned)((cols + 4 * kThreads - 1) / (4 * kThreads)));
+  const bool quads = cols % 4 == 0 && out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(part) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+  if (dtype == 1) sum_slots_kernel<__half><<<grid, kThreads, 0, st>>>(part, slots, cols, static_cast<__half*>(out), out_stride, quads);
+  else sum_slots_kernel<bf16><<<grid, kThreads, 0, st>>>(part, slots, cols, static_cast<bf16*>(out), out_stride, quads);
   return cudaGetLastError();
 }
 

@@ -58,6 +58,12 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same from zero
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -75,19 +81,20 @@ __device__ __forceinline__ uint32_t round_pair(float f0, float f1, __half) {
   const __half2 v = __floats2half2_rn(f0, f1);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// The leading bits of two floats as a bf16 pair, cut off (never rounded up to infinity), and what is left of them: of an infinity
-// nothing.
+// The leading bits of two floats as a bf16 pair, cut off (never rounded up to infinity), and what is left of them. FINITE: of
+// an infinity NaN is left, else nothing.
+template <bool FINITE>
 __device__ __forceinline__ uint32_t take_bf16(float& f0, float& f1) {
   const uint32_t b0 = __float_as_uint(f0) & 0xffff0000u, b1 = __float_as_uint(f1) & 0xffff0000u;
-  f0 = fabsf(f0) == INFINITY ? 0.f : f0 - __uint_as_float(b0);
-  f1 = fabsf(f1) == INFINITY ? 0.f : f1 - __uint_as_float(b1);
+  f0 = !FINITE && fabsf(f0) == INFINITY ? 0.f : f0 - __uint_as_float(b0);
+  f1 = !FINITE && fabsf(f1) == INFINITY ? 0.f : f1 - __uint_as_float(b1);
   return __byte_perm(b0, b1, 0x7632);
 }
 // N bf16 terms of the pair (f0, f1)
-template <int N>
+template <int N, bool FINITE = false>
 __device__ __forceinline__ void split(float f0, float f1, uint32_t (&t)[N]) {
 #pragma unroll
-  for (int i = 0; i < N - 1; i++) t[i] = take_bf16(f0, f1);
+  for (int i = 0; i < N - 1; i++) t[i] = take_bf16<FINITE>(f0, f1);
   t[N - 1] = round_bf16(f0, f1);
 }
 
@@ -124,6 +131,24 @@ __device__ __forceinline__ void mma_terms(float (&c)[4], const uint32_t (&a)[XN]
         if (i + j == s) mma(c, a[i], b0[j], b1[j], CT());
 }
 
+// the bf16 products by themselves, c = ...
+template <int XN, int PN>
+__device__ __forceinline__ void mma_terms_first(float (&c)[4], const uint32_t (&a)[XN][4], const uint32_t (&b0)[PN], const uint32_t (&b1)[PN]) {
+  constexpr int MOST = PN > XN ? PN : XN;
+  bool first = true;
+#pragma unroll
+  for (int s = MOST - 1; s >= 0; s--)
+#pragma unroll
+    for (int i = 0; i < XN; i++)
+#pragma unroll
+      for (int j = 0; j < PN; j++)
+        if (i + j == s) {
+          if (first) mma_first(c, a[i], b0[j], b1[j]);
+          else mma(c, a[i], b0[j], b1[j], bf16());
+          first = false;
+        }
+}
+
 // ---------------------------------------------------------------------------------------------------- shared-memory tiles
 // ROWS x COLS elements in chunks of 16 bytes; a row's chunks are permuted so that the eight rows of a matrix fragment, and eight
 // neighbouring chunks of a row, lie in different banks.
@@ -145,6 +170,10 @@ enum { kBy16 = 0, kBy8 = 1, kByElement = 2 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+// `bytes` of 16, the others zero
+__device__ __forceinline__ void cp16_sized(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
@@ -205,7 +234,7 @@ __device__ __forceinline__ void load_b(uint32_t base, int col0, int k0, uint32_t
           asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(f0) : "r"(W::at(base, k, c) + 4 * (i & 3)) : "memory");
           asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(f1) : "r"(W::at(base, k + 1, c) + 4 * (i & 3)) : "memory");
         }
-        split<TERMS>(f0, f1, b[t][h]);
+        split<TERMS, true>(f0, f1, b[t][h]);   // (an infinite float32 parameter makes NaN)
       }
   }
 }
@@ -378,17 +407,15 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
   const bool staged = a.base != nullptr && a.vec_out;   // the base's rows come with the weights
   const uint32_t ring = smem_at(smem);
 
-  // this thread's chunks: where they come from in the first stage of each product, and where they go
-  const XT *xp[XD::EACH], *yp[YD::EACH];
+  // This thread's chunks: where they come from in the first stage of each product, and where they go. A row or rank that does not
+  // exist is read as zero bytes of one that does.
+  const XT* xp[XD::EACH];
+  bool x_there[XD::EACH];
 #pragma unroll
   for (int k = 0; k < XD::EACH; k++) {
     const int e = s_row[XD::row() + k * XD::STEP];
-    xp[k] = e < 0 ? nullptr : static_cast<const XT*>(a.in) + (long long)(a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div)) * a.in_stride + b0 * KB;
-  }
-#pragma unroll
-  for (int k = 0; k < YD::EACH; k++) {
-    const int e = YD::has(k) ? s_row[YD::row() + k * YD::STEP] : -1;
-    yp[k] = e < 0 || !staged ? nullptr : static_cast<const XT*>(a.base) + (long long)e * a.base_stride + lo;
+    x_there[k] = e >= 0;
+    xp[k] = static_cast<const XT*>(a.in) + (long long)(e < 0 ? 0 : a.in_div == 1 ? e : (int)((unsigned)e / (unsigned)a.in_div)) * a.in_stride + b0 * KB;
   }
   const uint32_t x_to = XTile::at(0, XD::row(), XD::chunk()), w1_to = S::X + W1D::T::at(0, W1D::row(), W1D::chunk());
   const uint32_t y_to = YTile::at(0, YD::row(), YD::chunk());
@@ -396,47 +423,73 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
   const long long l1 = BWD ? a.r : a.D1, l2 = BWD ? a.D2 : a.r;
   const PT* p1 = w1 + (BWD ? (long long)b0 * KB * l1 : (long long)b0 * KB);
   const PT* p2 = w2 + (BWD ? (long long)lo : (long long)lo * l2);
+  // stages that have all of their contraction, or columns
+  const int full1 = FAST ? min(n1, a.D1 / KB - b0) : 0, full2 = FAST ? (hi - lo) / NB : 0;
+  // what the whole stages' weights are read by: of the ranks, those that exist
+  const PT* q1 = p1 + (!BWD && W1D::row() >= a.r ? 0 : W1D::row()) * l1 + (BWD && PerChunk<PS>() * W1D::chunk() >= a.r ? 0 : PerChunk<PS>() * W1D::chunk());
+  const PT* q2 = p2 + (BWD && W2D::row() >= a.r ? 0 : W2D::row()) * l2 + (!BWD && PerChunk<PS>() * W2D::chunk() >= a.r ? 0 : PerChunk<PS>() * W2D::chunk());
 
   int next = 0, into = 0;   // the stage to be fetched, its place in the ring
   auto fetch = [&]() {
     const uint32_t at = ring + into * S::STAGE;
     into = into + 1 == S::STAGES ? 0 : into + 1;
-    if (next < n1) {
+    if (next < full1) {
+#pragma unroll
+      for (int k = 0; k < XD::EACH; k++)
+        cp16_sized(at + x_to + k * XD::STEP * XTile::CHUNKS * 16, xp[k] + (next * KB + PerChunk<2>() * XD::chunk()), x_there[k] ? 16 : 0);
+      const PT* q = q1 + (BWD ? (long long)next * KB * l1 : (long long)next * KB);
+#pragma unroll
+      for (int k = 0; k < W1D::EACH; k++) {
+        const bool there = BWD ? PerChunk<PS>() * W1D::chunk() < a.r : W1D::row() + k * W1D::STEP < a.r;
+        if (W1D::has(k)) cp16_sized(at + w1_to + k * W1D::STEP * W1D::T::CHUNKS * 16, BWD || there ? q + k * (W1D::STEP * l1) : q1, there ? 16 : 0);
+      }
+    } else if (next < n1) {
       const int k0 = next * KB, left = a.D1 - b0 * KB - k0;   // of the contraction
 #pragma unroll
       for (int k = 0; k < XD::EACH; k++) {
         const int c = PerChunk<2>() * XD::chunk();
-        if constexpr (FAST) cp16(at + x_to + k * XD::STEP * XTile::CHUNKS * 16, xp[k] != nullptr && c < left ? xp[k] + k0 + c : static_cast<const XT*>(a.in), xp[k] != nullptr && c < left);
-        else load_chunk<2>(at + x_to + k * XD::STEP * XTile::CHUNKS * 16, xp[k] != nullptr ? xp[k] + k0 : a.in, c, xp[k] != nullptr ? left : 0, a.by_in);
+        load_chunk<2>(at + x_to + k * XD::STEP * XTile::CHUNKS * 16, x_there[k] ? xp[k] + k0 : a.in, c, x_there[k] ? left : 0, FAST ? kBy16 : a.by_in);
       }
 #pragma unroll
       for (int k = 0; k < W1D::EACH; k++) {
         if (!W1D::has(k)) continue;
         const int m = W1D::row() + k * W1D::STEP, c = PerChunk<PS>() * W1D::chunk();
-        const uint32_t to = at + w1_to + k * W1D::STEP * W1D::T::CHUNKS * 16;
         const PT* row = p1 + m * l1 + (BWD ? (long long)k0 * l1 : (long long)k0);
         const bool there = BWD ? m < left : m < a.r;
-        const int most = BWD ? a.r : left;
-        if constexpr (FAST) cp16(to, there && c < most ? row + c : w1, there && c < most);
-        else load_chunk<PS>(to, there ? row : w1, c, there ? most : 0, a.by_w1);
+        load_chunk<PS>(at + w1_to + k * W1D::STEP * W1D::T::CHUNKS * 16, there ? row : w1, c, there ? (BWD ? a.r : left) : 0, FAST ? kBy16 : a.by_w1);
       }
     } else if (next < n1 + n2) {
       const int c0 = (next - n1) * NB, left = hi - lo - c0;   // of the columns
+      if (next - n1 < full2) {
+        const PT* q = q2 + (BWD ? (long long)c0 : (long long)c0 * l2);
 #pragma unroll
-      for (int k = 0; k < W2D::EACH; k++) {
-        if (!W2D::has(k)) continue;
-        const int m = W2D::row() + k * W2D::STEP, c = PerChunk<PS>() * W2D::chunk();
-        const uint32_t to = at + S::Y + W2D::T::at(0, BWD ? m : place_of<CW>(m), W2D::chunk());
-        const PT* row = p2 + m * l2 + (BWD ? (long long)c0 : (long long)c0 * l2);
-        const bool there = BWD ? m < a.r : m < left;
-        const int most = BWD ? left : a.r;
-        if constexpr (FAST) cp16(to, there && c < most ? row + c : w2, there && c < most);
-        else load_chunk<PS>(to, there ? row : w2, c, there ? most : 0, a.by_w2);
+        for (int k = 0; k < W2D::EACH; k++) {
+          const int m = W2D::row() + k * W2D::STEP;
+          const bool there = BWD ? m < a.r : PerChunk<PS>() * W2D::chunk() < a.r;
+          const uint32_t to = W2D::STEP % CW == 0 ? W2D::T::at(0, BWD ? W2D::row() : place_of<CW>(W2D::row()), W2D::chunk()) + k * W2D::STEP * W2D::T::CHUNKS * 16
+                                                  : W2D::T::at(0, BWD ? m : place_of<CW>(m), W2D::chunk());
+          if (W2D::has(k)) cp16_sized(at + S::Y + to, !BWD || there ? q + k * (W2D::STEP * l2) : q2, there ? 16 : 0);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < W2D::EACH; k++) {
+          if (!W2D::has(k)) continue;
+          const int m = W2D::row() + k * W2D::STEP, c = PerChunk<PS>() * W2D::chunk();
+          const PT* row = p2 + m * l2 + (BWD ? (long long)c0 : (long long)c0 * l2);
+          const bool there = BWD ? m < a.r : m < left;
+          load_chunk<PS>(at + S::Y + W2D::T::at(0, BWD ? m : place_of<CW>(m), W2D::chunk()), there ? row : w2, c, there ? (BWD ? left : a.r) : 0,
+                         FAST ? kBy16 : a.by_w2);
+        }
       }
+      if (staged) {
+        const int c = c0 + PerChunk<2>() * YD::chunk();
 #pragma unroll
-      for (int k = 0; k < YD::EACH; k++) {
-        const int c = PerChunk<2>() * YD::chunk();
-        if (yp[k] != nullptr) cp16(at + y_to + k * YD::STEP * YTile::CHUNKS * 16, c < left ? yp[k] + c0 + c : yp[k], c < left);
+        for (int k = 0; k < YD::EACH; k++) {
+          if (!YD::has(k)) continue;
+          const int e = s_row[YD::row() + k * YD::STEP];
+          const bool there = e >= 0 && c < hi - lo;
+          cp16_sized(at + y_to + k * YD::STEP * YTile::CHUNKS * 16, static_cast<const XT*>(a.base) + (there ? (long long)e * a.base_stride + lo + c : 0), there ? 16 : 0);
+        }
       }
     }
     next++;
@@ -483,8 +536,8 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
               if constexpr (PS == 4) {
                 // The tensor cores cut off what a sum has below its last bit. Where float32 results are wanted, a step's products
                 // are added up by themselves and then, rounded, to the whole.
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_terms<XN, P1, CT>(part, xa[m], b[h][0], b[h][1]);
+                float part[4];
+                mma_terms_first<XN, P1>(part, xa[m], b[h][0], b[h][1]);
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[m][2 * n + h][c] += part[c];
               } else {
