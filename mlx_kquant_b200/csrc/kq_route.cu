@@ -6,13 +6,14 @@
 // w_j = scale * s_ij / (sum s_i + 1e-20), or scale * s_ij.
 //
 // A warp per token, a lane NI neighbouring experts, all in registers. The order is that of 64 bits; exponentials and sums in 64 bits
-// for all experts took 66 us for 16384 tokens of 256 experts, this kernel takes 13. It ranks 32-bit codes: what an expert is ranked
-// by in the upper bits (score + bias as fixed point over the range of the biases, or a logit's leading bits), its index, counted
-// down, in the lower ones. A lane sorts its codes, and each pick is one warp-wide maximum of the lanes' first. The codes' error is
-// bounded (kRouteSlack): where neighbours in the order of the picks, the last of them and the best that is left, or the sums around the
-// border of the groups lie no further apart than that, and are not the same logit and bias bit for bit, the token is ranked again in
-// 64 bits. A code holds all of a 16-bit logit: without a bias and sums nothing is ever ranked again. What is left is instruction
-// issue: some 450 a token.
+// for all experts took 66 us for 16384 tokens of 256 experts in 8 groups, this kernel takes 22. It ranks 32-bit codes: what an expert
+// is ranked by in the upper bits (score + bias as fixed point over the range of the biases, or a logit's leading bits), its index,
+// counted down, in the lower ones. A lane sorts its codes, and each pick is one warp-wide maximum of the lanes' first. The codes'
+// error is bounded (kRouteSlack): where neighbours in the order of the picks, the last of them and the best that is left, or the
+// sums around the border of the groups lie no further apart than that, and are not the same logit and bias bit for bit (one token
+// in 250 of normally distributed logits), the token is ranked again with 64 bits for its 32 best codes and for the experts that
+// count for the groups, and if that leaves a doubt with 64 bits for all (which one token alone takes 12 us for). A code holds all
+// of a 16-bit logit: without a bias and sums nothing is ever ranked again. What is left is instruction issue: some 800 a token.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -231,9 +232,11 @@ __device__ __forceinline__ void store_picks(const RouteArgs& a, int token, const
   float score = 0.f;
   if (win >= 0) {
     const float x = static_cast<float>(row[win]);
-    score = a.scoring == 0 ? expf(x - fm) / fz : rt_sigmoid(x);
+    // (quotients within two steps)
+    score = a.scoring == 0 ? __fdividef(expf(x - fm), fz) : __fdividef(1.f, 1.f + expf(-x));
+    if (a.scoring != 0 && x < -80.f) score = expf(x);   // (1 + e^-x beyond the range of that quotient)
   }
-  if (a.norm) score /= rt_sum(score) + 1e-20f;
+  if (a.norm) score = __fdividef(score, rt_sum(score) + 1e-20f);
   if (lane < a.top_k) {
     const long long at = (long long)token * a.top_k + lane;
     a.indices[at] = win;
@@ -313,7 +316,7 @@ __device__ __forceinline__ void merge_two(uint32_t c0, uint32_t c1, uint32_t& b0
 }
 
 template <int NI>
-constexpr int route_ctas() { return NI <= 4 ? 10 : NI == 8 ? 8 : NI == 16 ? 4 : 2; }   // of an SM
+constexpr int route_ctas() { return NI <= 4 ? 6 : NI == 8 ? 5 : NI == 16 ? 4 : 2; }   // of an SM: more of them spill
 
 template <typename T, int NI>
 __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kernel(const RouteArgs a) {
@@ -354,25 +357,36 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
   const int lanes = a.G > 1 ? a.size / NI : 1;   // of a group
   const bool whole_groups = a.G > 1 && a.G <= 32 && a.size % NI == 0 && 32 % lanes == 0;
 
-  // Up to 32 tokens at a time, then those of them that 64 bits have to rank: the registers are free by then.
+  // Up to 32 tokens at a time, then those of them that the codes could not rank: once more with 64 bits for the best 32 codes, and for
+  // the experts that count for the groups; and if that too leaves a doubt, with 64 bits for all.
   const int stride = gridDim.x * kRouteWarps;
-  int first = blockIdx.x * kRouteWarps + warp, it = 0;
+  int ahead = blockIdx.x * kRouteWarps + warp, first = ahead, it = 0;   // the next token; the first of these 32, how many of them
   uint32_t again = 0;
-  auto exactly = [&]() {
-    for (; again != 0; again &= again - 1) {
-      const int t = first + (__ffs(again) - 1) * stride;
-      route_exactly<T, NI>(a, t, static_cast<const T*>(a.logits) + (long long)t * a.E, grp, bits);
-    }
-  };
-  for (int token = first; token < a.T; token += stride, it++) {
-    if (it == 32) {
-      exactly();
-      first = token;
-      it = 0;
+  bool exactly = false;
+  for (;;) {
+    int token = ahead;
+    if (!exactly && (ahead >= a.T || it == 32)) exactly = true;
+    if (exactly) {
+      if (again == 0) {
+        if (ahead >= a.T) break;
+        exactly = false;
+        first = ahead;
+        it = 0;
+        continue;
+      }
+      token = first + (__ffs(again) - 1) * stride;
+      again &= again - 1;
+    } else {
+      ahead = ahead < a.T - stride ? ahead + stride : a.T;
     }
     const T* row = static_cast<const T*>(a.logits) + (long long)token * a.E;
-    float l[NI], s[NI];
+    if (exactly && a.scoring == 0 && groups_by_score && (by_score || a.G > 1)) {   // (the sum of the exponentials in 64 bits too)
+      route_exactly<T, NI>(a, token, row, grp, bits);
+      continue;
+    }
+    float l[NI];
     load_row<T, NI>(row, a.E, a.whole, l);
+    float s[NI];
     bool close = odd;
     float fm = 0.f, fz = 1.f;
     if (a.scoring == 0) {
@@ -384,12 +398,17 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
 #pragma unroll
       for (int i = 0; i < NI; i++) s[i] = fast_sigmoid(l[i]);
     }
-    // a NaN's code would not come first; scores that are not numbers 64 bits have to deal with
+    // a NaN's code would not come first; scores that are not numbers the full form has to deal with
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < NI; i++) nan |= l[i] != l[i];
     nan |= fz != fz;
     close |= __any_sync(kAll, nan);
+    auto score_of = [&](uint32_t code) {   // of an expert, in 64 bits (sigmoid)
+      const int e = (int)(IM - (code & IM));
+      const double v = 1. / (1. + exp(-(double)static_cast<float>(row[e])));
+      return by_score ? v + (double)a.bias[e] : v;
+    };
     uint32_t code[NI], by[NI];   // of the scores, and what experts are ranked by
     if (by_score || (a.G > 1 && groups_by_score)) {
 #pragma unroll
@@ -410,7 +429,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
         for (int o = 1; o < lanes; o <<= 1) merge_two(__shfl_xor_sync(kAll, b0, o), __shfl_xor_sync(kAll, b1, o), b0, b1);
         // lane g comes to have group g: what it counts, and its index counted down; none without an expert
         const uint32_t count = __shfl_sync(kAll, a.group_top > 1 ? (b0 >> IB) + (b1 >> IB) : b0 >> IB, lane * lanes & 31);
-        uint32_t mine = lane < a.G && count != 0 ? count << 5 | (31 - lane) : 0u, last = 0;
+        const uint32_t whole = lane < a.G && count != 0 ? count << 5 | (31 - lane) : 0u;
+        uint32_t mine = whole, last = 0;
         bool stays = false;
         for (int r = 0; r < a.top_groups; r++) {
           last = __reduce_max_sync(kAll, mine);
@@ -419,8 +439,33 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
             stays = true;
           }
         }
-        const uint32_t next = __reduce_max_sync(kAll, mine), kept = __ballot_sync(kAll, stays);
-        if (next != 0 && (sizeof(T) == 4 || groups_by_score)) close |= (last >> 5) - (next >> 5) <= groups_close_by;
+        const uint32_t next = __reduce_max_sync(kAll, mine);
+        if (next != 0 && (sizeof(T) == 4 || groups_by_score) && (last >> 5) - (next >> 5) <= groups_close_by) {
+          if (!exactly || !groups_by_score) {
+            close = true;
+          } else {
+            // the experts that count, if no other comes near them: their scores' sum
+            uint32_t third = 0;
+#pragma unroll
+            for (int i = 0; i < NI; i++)
+              if (code[i] < (a.group_top > 1 ? b1 : b0)) third = max(third, code[i]);
+            for (int o = 1; o < lanes; o <<= 1) third = max(third, __shfl_xor_sync(kAll, third, o));
+            close |= __any_sync(kAll, third != 0 && ((a.group_top > 1 ? b1 : b0) >> IB) - (third >> IB) <= unsure);
+            const uint32_t c0 = __shfl_sync(kAll, b0, lane * lanes & 31), c1 = __shfl_sync(kAll, b1, lane * lanes & 31);
+            double v = -INFINITY;
+            if (whole != 0) {
+              v = score_of(c0);
+              if (a.group_top > 1 && c1 != 0) v += score_of(c1);
+            }
+            int ahead = 0;
+            for (int h = 0; h < a.G; h++) {
+              const double o = __shfl_sync(kAll, v, h);
+              ahead += o > v || (o == v && h < lane);
+            }
+            stays = whole != 0 && ahead < a.top_groups;
+          }
+        }
+        const uint32_t kept = __ballot_sync(kAll, stays);
         if (!(kept >> (lane / lanes) & 1)) {
 #pragma unroll
           for (int i = 0; i < NI; i++) code[i] = by[i] = 0;
@@ -447,34 +492,52 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
     }
     sort_codes<NI>(by);
     uint32_t mine = 0;       // lane r: the r-th pick's code; one more, where it has to be told how near that comes
-    const int rounds = a.top_k < 32 && !sure ? a.top_k + 1 : a.top_k;
+    const int rounds = exactly ? 32 : sure ? a.top_k : min(32, a.top_k + 1);
     for (int r = 0; r < rounds; r++) {
       const uint32_t top = __reduce_max_sync(kAll, by[0]);
-      if (lane == r) mine = top;
-      if (by[0] == top) {
+      const bool took = by[0] == top;
+      mine = lane == r ? top : mine;
 #pragma unroll
-        for (int i = 0; i < NI - 1; i++) by[i] = by[i + 1];
-        by[NI - 1] = 0;
-      }
+      for (int i = 0; i < NI - 1; i++) by[i] = took ? by[i + 1] : by[i];   // (selected, not branched over)
+      by[NI - 1] = took ? 0u : by[NI - 1];
     }
-    if (!sure) {
+    int e = mine != 0 ? (int)(IM - (mine & IM)) : -1;
+    if (exactly) {
+      const uint32_t end = __shfl_sync(kAll, mine, 31), least = __shfl_sync(kAll, mine, a.top_k - 1);
+      close |= a.top_k == 32 || (end != 0 && (least >> IB) - (end >> IB) <= close_by);   // more than 32 come near
+      const double v = mine == 0 ? -INFINITY : by_score ? score_of(mine) : (double)static_cast<float>(row[e]);
+      int place = 0;
+      for (int h = 0; h < 32; h++) {
+        const double o = __shfl_sync(kAll, v, h);
+        const int f = __shfl_sync(kAll, e, h);
+        place += o > v || (o == v && f < e && f >= 0);
+      }
+      if (e < 0) place = 32;
+      int win = -1;
+      for (int h = 0; h < 32; h++) {
+        const int p = __shfl_sync(kAll, place, h), f = __shfl_sync(kAll, e, h);
+        if (p == lane) win = f;
+      }
+      e = win;
+    } else if (!sure) {
       const uint32_t before = __shfl_up_sync(kAll, mine, 1);
       const bool near = lane > 0 && mine != 0 && (before >> IB) - (mine >> IB) <= close_by;
       if (__any_sync(kAll, near)) {
         // equals in every bit keep the order of their indices; what follows the last one is not known
         bool same = false;
         if (near && lane < a.top_k) {
-          const int e = (int)(IM - (mine & IM)), f = (int)(IM - (before & IM));
+          const int f = (int)(IM - (before & IM));
           same = static_cast<float>(row[e]) == static_cast<float>(row[f]) && (!by_score || a.bias[e] == a.bias[f]);
         }
         close |= __any_sync(kAll, near && !same);
       }
       close |= a.top_k == 32;
     }
-    if (close) again |= 1u << it;
-    else store_picks<T>(a, token, row, lane < a.top_k && mine != 0 ? (int)(IM - (mine & IM)) : -1, fm, fz);
+    if (!close) store_picks<T>(a, token, row, lane < a.top_k ? e : -1, fm, fz);
+    else if (exactly) route_exactly<T, NI>(a, token, row, grp, bits);
+    else again |= 1u << it;
+    if (!exactly) it++;
   }
-  exactly();
 }
 
 // dl from dw. A warp per token; everything but the picks is zero, except with softmax scores that are not renormalised.

@@ -178,3 +178,20 @@ def test_rows_that_run_out_of_experts_reach_the_block(T):
     assert (y[0] == 0).all() and torch.isfinite(y).all()
     full = torch.where(idx < 0, 0, idx)            # weight 0 on some other expert
     torch.testing.assert_close(y.float(), moe_glu(x, wg, wu, wd, "q4_k", full, w).float(), rtol=0.02, atol=0.01)
+
+
+@pytest.mark.parametrize("group_top", [1, 2])
+def test_many_doubtful_tokens(group_top):
+    """Logits and biases of few values a hair apart, so that most tokens are ranked again, some with more than 32 experts in doubt."""
+    g = torch.Generator().manual_seed(group_top)
+    T, E, k = 700, 256, 8
+    for step, few in ((2.0 ** -22, 4), (2.0 ** -23, 2), (2.0 ** -18, 40)):
+        x = 0.75 + torch.randint(0, few, (T, E), generator=g) * step
+        x[::3] += torch.randn(x[::3].shape, generator=g)
+        bias = 0.125 + torch.randint(0, few, (E,), generator=g) * step * 0.5
+        case = (T, E, k, 8, 4, "sigmoid", True, group_top, True)
+        xd = x.double().numpy()
+        want, _, _ = route(xd, k, 8, 4, "sigmoid", bias.double().numpy(), group_top)
+        np.testing.assert_array_equal(run(x.cuda(), case, bias.cuda())[0].cpu().numpy(), want)
+        want, _, _ = route(xd, k, 8, 4, "sigmoid", None, group_top)
+        np.testing.assert_array_equal(run(x.cuda(), case, None)[0].cpu().numpy(), want)
