@@ -424,7 +424,8 @@ template <typename XT, typename PT, int RT, bool FAST, bool SHORT>
 cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
   typedef WgradShape<PT, RT, SHORT> S;
   auto kern = wgrad_kernel<XT, PT, RT, FAST, SHORT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  static bool done[16] = {};
+  const cudaError_t e = allow_smem(kern, S::SMEM, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((a.tiles + (a.of[1].out != nullptr ? (a.of[1].D + S::COLS - 1) / S::COLS : 0)) * cluster), (unsigned)a.n_groups, (unsigned)((a.r + 63) / 64));
@@ -483,8 +484,12 @@ __global__ void __launch_bounds__(kThreads) sum_slots_kernel(const float* part, 
 }
 
 int sm_count() {
+  static int known[16] = {};   // of the devices asked for so far
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 16 && known[dev] != 0) return known[dev];
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 16) known[dev] = sms;
   return sms;
 }
 
@@ -586,7 +591,8 @@ cudaError_t launch_lora_plan(const LoraGroups& g, void* plan, cudaStream_t st) {
   plan_count_kernel<<<l.chunks, kChunkThreads, 0, st>>>(g, n_groups, l.chunk, counts);
   const int smem = 32 * (n_groups + 1) * 2;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * kPlanKeys * 2);
+    static bool done[16] = {};
+    const cudaError_t e = allow_smem(plan_place_kernel, 32 * kPlanKeys * 2, done);
     if (e != cudaSuccess) return e;
   }
   plan_place_kernel<<<l.chunks, kChunkThreads, smem, st>>>(g, n_groups, l.chunk, l.tile_rows, counts, order, offsets, tiles);

@@ -35,7 +35,7 @@ constexpr int kThreads = 256;
 __device__ __forceinline__ int group_of(const LoraGroups& g, long long e) {
   int id = 0;
   if (g.ids != nullptr) {
-    id = g.ids[e / g.slots];
+    id = g.ids[g.slots == 1 ? (unsigned)e : (unsigned)e / (unsigned)g.slots];
     if ((unsigned)id >= (unsigned)g.G) return -1;
   }
   if (g.experts == nullptr) return id;
@@ -251,22 +251,30 @@ __device__ __forceinline__ TileAt find_tile(const LoraArgs& a, int tile, int* s_
   TileAt t;
   if (a.direct) {
     if (tid < 32) {
+      // the groups of up to 128 entries at once; longer calls in turns
+      const int n = (int)a.g.n;
       const int mine = group_of(a.g, tile);
-      int before = 0;
-      for (int b = tid; b < tile; b += 32) before += group_of(a.g, b) == mine;
+      int before = 0, rows = 0;
+      for (int b0 = 0; b0 < n; b0 += 128) {
+        int key[4];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      int rows = 0;
-      if (before % MT == 0) {
-        for (int b0 = tile; b0 < (int)a.g.n && rows < MT; b0 += 32) {
-          const int b = b0 + tid;
-          const bool same = b < (int)a.g.n && group_of(a.g, b) == mine;
-          const uint32_t m = __ballot_sync(0xffffffffu, same);
-          const int at = rows + __popc(m & ((1u << tid) - 1u));
-          if (same && at < MT) s_row[at] = b;
-          rows = min(MT, rows + __popc(m));
+        for (int k = 0; k < 4; k++) {
+          const int b = b0 + 32 * k + tid;
+          key[k] = b < n ? group_of(a.g, b) : -2;
         }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int b = b0 + 32 * k + tid, left = tile - (b0 + 32 * k);   // entries of these 32 that lie ahead of the cluster's own
+          const uint32_t m = __ballot_sync(0xffffffffu, key[k] == mine), ahead = left <= 0 ? 0u : left >= 32 ? ~0u : (1u << left) - 1u;
+          before += __popc(m & ahead);
+          const uint32_t from = m & ~ahead;
+          const int at = rows + __popc(from & ((1u << tid) - 1u));
+          if ((from >> tid & 1) && at < MT) s_row[at] = b;
+          rows = min(MT, rows + __popc(from));
+        }
+        if (b0 + 128 > tile && (before % MT != 0 || rows == MT)) break;
       }
+      if (before % MT != 0) rows = 0;   // another cluster's
       for (int i = rows + tid; i < MT; i += 32) s_row[i] = -1;
       if (tid == 0) {
         s_info[0] = mine;
@@ -771,12 +779,24 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
   if (a.shrink && C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
+// A kernel's shared memory, asked for once on each device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kern, int bytes, bool (&done)[16]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev >= 0 && dev < 16 && done[dev])) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 16) done[dev] = true;
+  return e;
+}
+
 template <typename XT, typename PT, bool BWD, int RT, int MT, bool FAST>
 cudaError_t launch_tile(const LoraArgs& a, int cluster, cudaStream_t st) {
   constexpr int smem = Shape<PT, BWD, RT, MT>::SMEM;
   auto kern = tile_kernel<XT, PT, BWD, RT, MT, FAST>;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static bool done[16] = {};
+    const cudaError_t e = allow_smem(kern, smem, done);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
