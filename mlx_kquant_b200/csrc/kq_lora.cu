@@ -17,6 +17,7 @@ constexpr int kPlanThreads = 512;
 // slots from start / height + group on, which no two groups share; slots that are left over hold none. 32768 entries of 256 groups
 // PLAN_TIME us, of which the 33 MB that the CTAs read from L2 are the most.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const LoraGroups g, int n_groups, int height, int* order, int* offsets, LoraTile* tiles) {
+  wait_for_launch();
   constexpr int WARPS = kPlanThreads / 32;
   __shared__ int s_less[WARPS], s_same[WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mine = blockIdx.x;
@@ -132,6 +133,7 @@ __device__ __forceinline__ int key_of(const LoraGroups& g, int e, int n_groups) 
 }
 
 __global__ void __launch_bounds__(kChunkThreads) plan_count_kernel(const LoraGroups g, int n_groups, int per, int* counts) {
+  wait_for_launch();
   __shared__ int s_count[kPlanKeys];
   const int n = (int)g.n, e0 = blockIdx.x * per, e1 = min(n, e0 + per);
   s_count[threadIdx.x] = 0;
@@ -143,6 +145,7 @@ __global__ void __launch_bounds__(kChunkThreads) plan_count_kernel(const LoraGro
 
 __global__ void __launch_bounds__(kChunkThreads) plan_place_kernel(const LoraGroups g, int n_groups, int per, int height, const int* counts, int* order,
                                                                    int* offsets, LoraTile* tiles) {
+  wait_for_launch();
   __shared__ int s_base[kPlanKeys], s_warp[32];
   extern __shared__ uint16_t s_rank[];   // [32 warps][n_groups + 1]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = (int)g.n, me = blockIdx.x, chunks = gridDim.x, keys = n_groups + 1;
@@ -229,6 +232,7 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && SHORT ? 4 : RT <= 2 ? 2 :
   typedef Tile<S::COLS, 2> InTile;
   typedef Tile<RP, 2> UvTile;
   extern __shared__ __align__(16) uint8_t smem[];
+  wait_for_launch();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, q = lane & 3, cq = warp & 3, half = warp >> 2;
@@ -427,17 +431,8 @@ cudaError_t wgrad_launch(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
   static bool done[16] = {};
   const cudaError_t e = allow_smem(kern, S::SMEM, done);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.tiles + (a.of[1].out != nullptr ? (a.of[1].D + S::COLS - 1) / S::COLS : 0)) * cluster), (unsigned)a.n_groups, (unsigned)((a.r + 63) / 64));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = S::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)cluster, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, a);
+  const int tiles = a.tiles + (a.of[1].out != nullptr ? (a.of[1].D + S::COLS - 1) / S::COLS : 0);
+  return launch(kern, dim3((unsigned)(tiles * cluster), (unsigned)a.n_groups, (unsigned)((a.r + 63) / 64)), kThreads, S::SMEM, cluster, st, a);
 }
 template <typename XT, typename PT, int RT, bool FAST>
 cudaError_t wgrad_length(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
@@ -458,6 +453,7 @@ cudaError_t wgrad_read(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
 // four neighbouring columns of a token a thread; part's rows are whole fours where `quads`
 template <typename XT>
 __global__ void __launch_bounds__(kThreads) sum_slots_kernel(const float* part, int slots, int cols, XT* out, long long out_stride, bool quads) {
+  wait_for_launch();
   const long long token = blockIdx.x;
   const int c = 4 * (blockIdx.y * kThreads + threadIdx.x);
   if (c >= cols) return;
@@ -585,18 +581,16 @@ cudaError_t launch_lora_plan(const LoraGroups& g, void* plan, cudaStream_t st) {
   int *order = reinterpret_cast<int*>(p + l.order), *offsets = reinterpret_cast<int*>(p + l.offsets), *counts = reinterpret_cast<int*>(p + l.counts);
   LoraTile* tiles = reinterpret_cast<LoraTile*>(p + l.tiles);
   if (l.chunks == 0) {
-    plan_kernel<<<n_groups + 1, kPlanThreads, 0, st>>>(g, n_groups, l.tile_rows, order, offsets, tiles);
-    return cudaGetLastError();
+    return launch(plan_kernel, dim3((unsigned)n_groups + 1), kPlanThreads, 0, 0, st, g, n_groups, l.tile_rows, order, offsets, tiles);
   }
-  plan_count_kernel<<<l.chunks, kChunkThreads, 0, st>>>(g, n_groups, l.chunk, counts);
+  cudaError_t e = launch(plan_count_kernel, dim3((unsigned)l.chunks), kChunkThreads, 0, 0, st, g, n_groups, l.chunk, counts);
+  if (e != cudaSuccess) return e;
   const int smem = 32 * (n_groups + 1) * 2;
   if (smem > 40 * 1024) {
     static bool done[16] = {};
-    const cudaError_t e = allow_smem(plan_place_kernel, 32 * kPlanKeys * 2, done);
-    if (e != cudaSuccess) return e;
+    if ((e = allow_smem(plan_place_kernel, 32 * kPlanKeys * 2, done)) != cudaSuccess) return e;
   }
-  plan_place_kernel<<<l.chunks, kChunkThreads, smem, st>>>(g, n_groups, l.chunk, l.tile_rows, counts, order, offsets, tiles);
-  return cudaGetLastError();
+  return launch(plan_place_kernel, dim3((unsigned)l.chunks), kChunkThreads, smem, 0, st, g, n_groups, l.chunk, l.tile_rows, counts, order, offsets, tiles);
 }
 
 cudaError_t launch_lora_wgrad(const LoraWgradArgs& a, int in_dtype, int out_f32, int cluster, cudaStream_t st) {
@@ -608,9 +602,8 @@ cudaError_t launch_lora_sum_slots(const float* part, int slots, long long tokens
                                   cudaStream_t st) {
   const dim3 grid((unsigned)tokens, (unsigned)((cols + 4 * kThreads - 1) / (4 * kThreads)));
   const bool quads = cols % 4 == 0 && out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(part) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
-  if (dtype == 1) sum_slots_kernel<__half><<<grid, kThreads, 0, st>>>(part, slots, cols, static_cast<__half*>(out), out_stride, quads);
-  else sum_slots_kernel<bf16><<<grid, kThreads, 0, st>>>(part, slots, cols, static_cast<bf16*>(out), out_stride, quads);
-  return cudaGetLastError();
+  if (dtype == 1) return launch(sum_slots_kernel<__half>, grid, kThreads, 0, 0, st, part, slots, cols, static_cast<__half*>(out), out_stride, quads);
+  return launch(sum_slots_kernel<bf16>, grid, kThreads, 0, 0, st, part, slots, cols, static_cast<bf16*>(out), out_stride, quads);
 }
 
 cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_stride, void* out, long long out_stride, void* u,

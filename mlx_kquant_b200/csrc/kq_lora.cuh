@@ -31,6 +31,29 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int kThreads = 256;
 
+// First in every kernel here: they are launched beside the end of the launch before them and wait for it, and let the next one start
+// likewise only then (so that what lies further back has ended for it too).
+__device__ __forceinline__ void wait_for_launch() {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;\n" ::: "memory");
+}
+// cluster: CTAs of a cluster, or 0
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kern)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, Params(args)...);
+}
+
 // ---------------------------------------------------------------------------------------------------- groups
 __device__ __forceinline__ int group_of(const LoraGroups& g, long long e) {
   int id = 0;
@@ -390,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
   float* s_factor = reinterpret_cast<float*>(s_u + S::U / 2);             // [MT]
   int* s_row = reinterpret_cast<int*>(s_factor + MT);                     // [MT]
   int* s_info = s_row + MT;
+  wait_for_launch();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, q = lane & 3;
@@ -799,17 +823,7 @@ cudaError_t launch_tile(const LoraArgs& a, int cluster, cudaStream_t st) {
     const cudaError_t e = allow_smem(kern, smem, done);
     if (e != cudaSuccess) return e;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.n_clusters * cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)cluster, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, a);
+  return launch(kern, dim3((unsigned)(a.n_clusters * cluster)), kThreads, smem, cluster, st, a);
 }
 template <typename XT, typename PT, bool BWD, int RT>
 cudaError_t launch_mt(const LoraArgs& a, int mt, int cluster, cudaStream_t st) {

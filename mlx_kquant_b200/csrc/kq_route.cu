@@ -324,6 +324,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
   constexpr uint32_t IM = (1u << IB) - 1;
   constexpr float UNITS = (float)(1ull << (32 - IB)) - 1024.f;
   extern __shared__ double route_smem[];   // per warp, with groups: what they count, E keys, bits
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;\n" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = NI * lane;
   double* grp = route_smem + (size_t)warp * (a.G + a.E + 16);
   uint32_t* bits = reinterpret_cast<uint32_t*>(grp + a.G + a.E);
@@ -543,6 +544,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
 // dl from dw. A warp per token; everything but the picks is zero, except with softmax scores that are not renormalised.
 template <typename T, int NI>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(const RouteArgs a) {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;\n" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int token = blockIdx.x * kRouteWarps + warp;
   if (token >= a.T) return;
@@ -609,6 +611,21 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(const 
     if (e0 + i < a.E) out[e0 + i] = static_cast<T>(d[i]);
 }
 
+// beside the end of the launch before it, for which the kernels wait
+cudaError_t route_go(void (*kern)(const RouteArgs), unsigned grid, size_t smem, const RouteArgs& a, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(32 * kRouteWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
 template <typename T, int NI>
 cudaError_t route_launch(RouteArgs& a, cudaStream_t st) {
   const unsigned grid = (unsigned)((a.T + kRouteWarps - 1) / kRouteWarps);
@@ -617,8 +634,7 @@ cudaError_t route_launch(RouteArgs& a, cudaStream_t st) {
   const uintptr_t all = reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.dlogits) | (uintptr_t)(a.E * sizeof(T));
   a.whole = a.E % NI == 0 && all % STEP == 0;
   if (a.dlogits != nullptr) {
-    route_backward_kernel<T, NI><<<grid, 32 * kRouteWarps, 0, st>>>(a);
-    return cudaGetLastError();
+    return route_go(route_backward_kernel<T, NI>, grid, 0, a, st);
   }
   a.whole_bias = a.E % NI == 0 && (reinterpret_cast<uintptr_t>(a.bias) | (uintptr_t)(a.E * 4)) % (NI == 2 ? 8 : 16) == 0;
   a.size = a.E / a.G;
@@ -633,8 +649,7 @@ cudaError_t route_launch(RouteArgs& a, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(route_kernel<T, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  route_kernel<T, NI><<<grid < room ? grid : room, 32 * kRouteWarps, smem, st>>>(a);
-  return cudaGetLastError();
+  return route_go(route_kernel<T, NI>, grid < room ? grid : room, smem, a, st);
 }
 template <typename T>
 cudaError_t route_width(RouteArgs& a, cudaStream_t st) {
