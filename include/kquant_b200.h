@@ -384,7 +384,8 @@ KQ_API int kq_lora_update(const void* x, int dtype, long long rows, int K, long 
                           long long y_row_stride, void* out, long long out_row_stride, void* saved, const void* plan,
                           size_t plan_bytes, void* stream);
 KQ_API size_t kq_lora_saved_bytes(long long rows, int rank, int param_dtype);
-KQ_API size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int rank, int param_dtype);
+KQ_API size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int N, int rank,
+                                               int param_dtype);
 KQ_API int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long dy_row_stride, const void* x, int K,
                             long long x_row_stride, int slots, int x_shared, const void* a, const void* b, int param_dtype,
                             int rank, int n_adapters, int n_experts, const int32_t* adapter_ids, const uint32_t* experts,

@@ -152,9 +152,9 @@ size_t kq_lora_saved_bytes(long long rows, int rank, int param_dtype) {
   return rows < 0 || rank < 1 || rank > kq::kLoraMaxRank ? 0 : kq::lora_saved_bytes(rows, rank, param_dtype == KQ_F32);
 }
 
-size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int rank, int param_dtype) {
-  return rows < 0 || slots < 1 || K < 1 || rank < 1 || rank > kq::kLoraMaxRank
-             ? 0 : kq::lora_backward_workspace_bytes(rows, slots, x_shared, K, rank, param_dtype == KQ_F32);
+size_t kq_lora_backward_workspace_bytes(long long rows, int slots, int x_shared, int K, int N, int rank, int param_dtype) {
+  return rows < 0 || slots < 1 || K < 1 || N < 1 || rank < 1 || rank > kq::kLoraMaxRank
+             ? 0 : kq::lora_backward_workspace_bytes(rows, slots, x_shared, K, N, rank, param_dtype == KQ_F32);
 }
 
 int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long dy_row_stride, const void* x, int K, long long x_row_stride,
@@ -176,7 +176,7 @@ int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long
   if (!dy || !a || !b || (da && !x) || (db && !u)) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] null pointer.", op);
   if ((adapter_ids != nullptr || experts != nullptr) && plan == nullptr)
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] needs the plan of its indices.", op);
-  if (workspace == nullptr || workspace_bytes < kq_lora_backward_workspace_bytes(rows, slots, x_shared, K, rank, param_dtype))
+  if (workspace == nullptr || workspace_bytes < kq_lora_backward_workspace_bytes(rows, slots, x_shared, K, N, rank, param_dtype))
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] workspace is smaller than kq_lora_backward_workspace_bytes.", op);
   const kq::LoraCall c{types_of(dtype, param_dtype), kq::LoraGroups{adapter_ids, experts, slots, n_adapters, n_experts, rows, scaling, scale},
                        x, x_row_stride, x_shared, K, N, rank, a, b, plan};

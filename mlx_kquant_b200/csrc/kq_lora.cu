@@ -450,6 +450,15 @@ cudaError_t wgrad_read(const LoraWgradArgs& a, int cluster, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------------- sum over slots
+// Rows that start anywhere, again at 16-byte boundaries, zero behind their end: two products read them.
+__global__ void __launch_bounds__(kThreads) align_rows_kernel(const uint16_t* in, long long in_stride, int cols, uint16_t* out, int out_stride) {
+  wait_for_launch();
+  const uint16_t* p = in + (long long)blockIdx.x * in_stride;
+  uint16_t* o = out + (long long)blockIdx.x * out_stride;
+#pragma unroll 8
+  for (int c = threadIdx.x; c < out_stride; c += kThreads) o[c] = c < cols ? p[c] : (uint16_t)0;
+}
+
 // four neighbouring columns of a token a thread; part's rows are whole fours where `quads`
 template <typename XT>
 __global__ void __launch_bounds__(kThreads) sum_slots_kernel(const float* part, int slots, int cols, XT* out, long long out_stride, bool quads) {
@@ -549,7 +558,7 @@ void set_reads(LoraArgs& a, const LoraCall& c, bool backward) {
   a.by_in = by(a.in, a.in_stride, a.D1, 2);
   a.by_w1 = by(a.w1, l1, l1, ps);
   a.by_w2 = by(a.w2, l2, l2, ps);
-  a.vec_out = by(a.out, a.out_stride, a.D2, 2) == kBy16 && (a.base == nullptr || by(a.base, a.base_stride, a.D2, 2) == kBy16);
+  a.by_out = std::max(by(a.out, a.out_stride, a.D2, 2), a.base != nullptr ? by(a.base, a.base_stride, a.D2, 2) : (int)kBy16);
   a.ru = (a.r + 7) / 8 * 8;
 }
 
@@ -637,8 +646,9 @@ static int slot_columns(long long n, int K) {
 }
 size_t lora_saved_bytes(long long n, int r, int param_f32) { return (size_t)n * ((r + 7) / 8 * 8) * (param_f32 ? 6 : 4); }
 static size_t v_bytes(long long n, int r, int f32) { return (lora_saved_bytes(n, r, f32) + 255) & ~(size_t)255; }
-size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int r, int param_f32) {
-  return v_bytes(n, r, param_f32) + (shared && slots > 1 ? (size_t)n * slot_columns(n, K) * 4 : 0);
+static size_t aligned_bytes(long long n, int N) { return N % 8 != 0 ? ((size_t)n * ((N + 7) / 8 * 8) * 2 + 255) & ~(size_t)255 : 0; }
+size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int N, int r, int param_f32) {
+  return v_bytes(n, r, param_f32) + aligned_bytes(n, N) + (shared && slots > 1 ? (size_t)n * slot_columns(n, K) * 4 : 0);
 }
 
 cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy_stride, const void* u, void* dx, long long dx_stride,
@@ -649,6 +659,14 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
   const bool summed = c.shared && c.g.slots > 1;
   const int f16 = c.types == kLoraF16 || c.types == kLoraF16F32, f32 = c.types == kLoraBf16F32 || c.types == kLoraF16F32;
   uint16_t* v = static_cast<uint16_t*>(workspace);
+  if (c.N % 8 != 0) {
+    uint16_t* aligned = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + v_bytes(c.g.n, c.r, f32));
+    const int stride = (c.N + 7) / 8 * 8;
+    if ((e = launch(align_rows_kernel, dim3((unsigned)c.g.n), kThreads, 0, 0, st, static_cast<const uint16_t*>(dy), dy_stride, c.N, aligned, stride)) != cudaSuccess)
+      return e;
+    dy = aligned;
+    dy_stride = stride;
+  }
   a.r = c.r;
   const int mt = set_rows(a, c, cluster);
   a.in = dy;
@@ -663,7 +681,7 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
   a.shrink = 1;
   a.scale_u = 1;
   const long long tokens = c.g.n / c.g.slots;
-  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(c.g.n, c.r, f32));
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(c.g.n, c.r, f32) + aligned_bytes(c.g.n, c.N));
   const int step = slot_columns(c.g.n, c.K);
   // a token's slots share its row: their parts in float32, as many columns at a time as stay in L2, then the sum
   auto columns = [&](int c0) {
@@ -680,6 +698,7 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
     a.out_stride = dx_stride;
   }
   set_reads(a, c, true);
+  if (c.N % 8 != 0) a.by_in = kBy16;   // (the rows put at boundaries above)
   if (dx != nullptr || da != nullptr) {
     if ((e = tile_launch(c.types, a, true, mt, cluster, st)) != cudaSuccess) return e;
   }
@@ -690,13 +709,14 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
       if ((c0 = a.c1) >= c.K) break;
       a.shrink = 0;
       columns(c0);
-      set_reads(a, c, true);
+      set_reads(a, c, true);   // (the rows are not read again)
       if ((e = tile_launch(c.types, a, true, mt, cluster, st)) != cudaSuccess) return e;
     }
   }
   if (da == nullptr && db == nullptr) return cudaSuccess;
   auto side = [&](const void* in, long long stride, int div, int D, const void* uv, int scaled, void* out, int r_first) {
-    return LoraWgrad{in, stride, div, D, static_cast<const uint16_t*>(uv), scaled, out, r_first, by(in, stride, D, 2)};
+    // (dy's rows are zero up to their own stride where they were put at boundaries)
+    return LoraWgrad{in, stride, div, D, static_cast<const uint16_t*>(uv), scaled, out, r_first, by(in, stride, in == dy && D % 8 != 0 ? (int)stride : D, 2)};
   };
   LoraWgradArgs w{};
   w.g = c.g;

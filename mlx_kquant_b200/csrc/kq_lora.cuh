@@ -326,25 +326,31 @@ __device__ __forceinline__ TileAt find_tile(const LoraArgs& a, int tile, int* s_
 template <typename XT>
 __device__ __forceinline__ float to_float(XT v) { return static_cast<float>(v); }
 
-// rows without an adapter: the base as it is
-template <typename XT>
-__device__ __forceinline__ void copy_rows(const LoraArgs& a, const int* s_row, int rows, int lo, int hi) {
-  if (a.out == nullptr || (a.out == a.base && !a.out_f32)) return;
-  for (int m = 0; m < rows; m++) {
-    const int row = s_row[m];
-    if (a.out_f32) {
-      float* o = static_cast<float*>(a.out) + (long long)row * a.out_stride - a.c0;
-      for (int c = lo + threadIdx.x; c < hi; c += kThreads) o[c] = 0.f;
-      continue;
-    }
-    XT* o = static_cast<XT*>(a.out) + (long long)row * a.out_stride - a.c0;
-    const XT* b = static_cast<const XT*>(a.base) + (long long)row * a.base_stride - a.c0;
-    if (a.vec_out) {
-      for (int c = lo + 8 * threadIdx.x; c < hi; c += 8 * kThreads)
-        *reinterpret_cast<uint4*>(o + c) = a.base != nullptr ? *reinterpret_cast<const uint4*>(b + c) : make_uint4(0, 0, 0, 0);
-    } else {
-      for (int c = lo + threadIdx.x; c < hi; c += kThreads) o[c] = a.base != nullptr ? b[c] : XT(0.f);
-    }
+// Rows without an adapter: columns [lo, hi) of the base as they are, zeros without one. A warp a row, eight accesses of a lane on their
+// way at once, of 16 bytes wherever the row starts (as long as base and out start alike).
+static __device__ __noinline__ void copy_rows(const uint16_t* base, long long base_stride, uint16_t* out, long long out_stride, const int* s_row, int rows, int lo,
+                                       int hi) {
+  const int lane = threadIdx.x & 31;
+  for (int m = threadIdx.x >> 5; m < rows; m += kThreads / 32) {
+    const uint16_t* p = base == nullptr ? nullptr : base + (long long)s_row[m] * base_stride + lo;
+    uint16_t* o = out + (long long)s_row[m] * out_stride + lo;
+    const int n = hi - lo;
+    const bool alike = p == nullptr || ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
+    const int head = alike ? min(n, (int)((16 - (reinterpret_cast<uintptr_t>(o) & 15)) & 15) / 2) : n, body = (n - head) / 8;
+    auto some = [&](auto* to, const auto* from, int count) {
+      for (int v0 = lane; v0 < count; v0 += 256) {
+        typename std::remove_reference<decltype(*to)>::type u[8] = {};
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (v0 + 32 * k < count && base != nullptr) u[k] = from[v0 + 32 * k];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (v0 + 32 * k < count) to[v0 + 32 * k] = u[k];
+      }
+    };
+    some(o, p, head);
+    some(reinterpret_cast<uint4*>(o + head), reinterpret_cast<const uint4*>(p + head), body);
+    some(o + head + 8 * body, p + head + 8 * body, n - head - 8 * body);
   }
 }
 
@@ -392,7 +398,7 @@ __device__ __forceinline__ int place_of(int n) {
   else return (n & ~15) | (n >> 1 & 1) << 3 | (n >> 2 & 3) << 1 | (n & 1);
 }
 
-// FAST: all rows are whole aligned groups of 16 bytes.
+// FAST: all rows that are read, and the forward pass' outputs, are whole aligned groups of 16 bytes.
 template <typename XT, typename PT, bool BWD, int RT, int MT, bool FAST>
 __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_kernel(const LoraArgs a) {
   typedef Shape<PT, BWD, RT, MT> S;
@@ -424,7 +430,12 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
   const int lo = a.c0 + n_chunks * rank / C * NB;
   const int hi = min(a.c1, a.c0 + n_chunks * (rank + 1) / C * NB);
   if (t.group < 0) {
-    copy_rows<XT>(a, s_row, t.rows, lo, hi);
+    if (a.out_f32) {
+      for (int m = warp; m < t.rows; m += kThreads / 32)
+        for (int c = lo + lane; c < hi; c += 32) static_cast<float*>(a.out)[(long long)s_row[m] * a.out_stride + c - a.c0] = 0.f;
+    } else if (a.out != nullptr && a.out != a.base) {
+      copy_rows(static_cast<const uint16_t*>(a.base), a.base_stride, static_cast<uint16_t*>(a.out), a.out_stride, s_row, t.rows, lo, hi);
+    }
     if (a.shrink && a.u != nullptr && rank == 0)
       for (int v = tid; v < t.rows * UT * a.ru; v += kThreads)
         a.u[((long long)(v / a.ru % UT) * a.g.n + s_row[v / (a.ru * UT)]) * a.ru + v % a.ru] = 0;
@@ -436,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
   const int blocks = a.shrink ? (a.D1 + KB - 1) / KB : 0;
   const int b0 = blocks * rank / C, n1 = blocks * (rank + 1) / C - b0;
   const int n2 = a.out != nullptr ? (hi - lo + NB - 1) / NB : 0;
-  const bool staged = a.base != nullptr && a.vec_out;   // the base's rows come with the weights
+  const bool staged = a.base != nullptr && a.by_out != kByElement;   // the base's rows come with the weights
   const uint32_t ring = smem_at(smem);
 
   // This thread's chunks: where they come from in the first stage of each product, and where they go. A row or rank that does not
@@ -522,7 +533,10 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
           if (!YD::has(k)) continue;
           const int e = s_row[YD::row() + k * YD::STEP];
           const bool there = e >= 0 && c < hi - lo;
-          cp16_sized(at + y_to + k * YD::STEP * YTile::CHUNKS * 16, static_cast<const XT*>(a.base) + (there ? (long long)e * a.base_stride + lo + c : 0), there ? 16 : 0);
+          const uint32_t to = at + y_to + k * YD::STEP * YTile::CHUNKS * 16;
+          const XT* row = static_cast<const XT*>(a.base) + (there ? (long long)e * a.base_stride + lo : 0);
+          if (FAST || a.by_out == kBy16) cp16_sized(to, row + (there ? c : 0), there ? 16 : 0);
+          else load_chunk<2>(to, row, c, there ? hi - lo : 0, kBy8);
         }
       }
     }
@@ -727,12 +741,12 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
           // columns c0 + cw + (CW / 4) q .. of two rows
           constexpr int HOLD = CW / 4;
           const int col = c0 + cw + HOLD * q;
+          const float (&c)[CW / 8][4] = acc[m];
+          if (FAST || a.by_out != kByElement) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            if (row[h] < 0 || col >= hi) continue;
-            const float (&c)[CW / 8][4] = acc[m];
-            XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride + col;
-            if (a.vec_out) {
+            for (int h = 0; h < 2; h++) {
+              if (row[h] < 0 || col >= hi) continue;
+              XT* o = static_cast<XT*>(a.out) + (long long)row[h] * a.out_stride + col;
               uint32_t v[HOLD / 2];
               const uint32_t p = YTile::at(at, m1 + 8 * h, (cw + HOLD * q) / 8) + (HOLD == 4 ? 8 * (q & 1) : 0);
               if constexpr (HOLD == 8) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(p) : "memory");
@@ -742,13 +756,43 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
                 const XT* y = reinterpret_cast<const XT*>(&v[n]);
                 v[n] = round_pair(fmaf(f[h], c[n][2 * h], to_float(y[0])), fmaf(f[h], c[n][2 * h + 1], to_float(y[1])), XT());
               }
-              if constexpr (HOLD == 8) *reinterpret_cast<uint4*>(o) = make_uint4(v[0], v[1], v[2], v[3]);
-              else *reinterpret_cast<uint2*>(o) = make_uint2(v[0], v[1]);
-            } else {
-              const XT* y = static_cast<const XT*>(a.base) + (long long)row[h] * a.base_stride + col;
+              if constexpr (HOLD == 8) {
+                if (FAST || a.by_out == kBy16) {
+                  *reinterpret_cast<uint4*>(o) = make_uint4(v[0], v[1], v[2], v[3]);
+                } else {
+                  *reinterpret_cast<uint2*>(o) = make_uint2(v[0], v[1]);
+                  if (col + 4 < hi) *reinterpret_cast<uint2*>(o + 4) = make_uint2(v[2], v[3]);
+                }
+              } else {
+                *reinterpret_cast<uint2*>(o) = make_uint2(v[0], v[1]);
+              }
+            }
+          } else {
+            // Rows that start anywhere: through shared memory in float32, eight rows at a time, to a column a lane, so that an access
+            // is a run of a row.
+            const int own = c0 + cw + (lane & (CW - 1));
+            constexpr int TURN = 32 / CW;   // rows at once
+            float* tile = reinterpret_cast<float*>(smem + (at - ring)) + warp * 8 * CW;
+            static_assert(kThreads / 32 * 8 * CW * 4 <= S::Y, "the stage's room for rows");
+            float y[2][8 / TURN];
 #pragma unroll
-              for (int n = 0; n < HOLD; n++)
-                if (col + n < hi) o[n] = XT(fmaf(f[h], c[n / 2][2 * h + n % 2], to_float(y[n])));
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+              for (int r = 0; r < 8 / TURN; r++) {
+                const int e = s_row[m0 + 16 * m + 8 * h + r * TURN + lane / CW];
+                y[h][r] = e >= 0 && own < hi ? to_float(static_cast<const XT*>(a.base)[(long long)e * a.base_stride + own]) : 0.f;
+              }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+              for (int n = 0; n < CW / 8; n++) *reinterpret_cast<float2*>(tile + i * CW + HOLD * q + 2 * n) = make_float2(f[h] * c[n][2 * h], f[h] * c[n][2 * h + 1]);
+              __syncwarp();
+#pragma unroll
+              for (int r = 0; r < 8 / TURN; r++) {
+                const int e = s_row[m0 + 16 * m + 8 * h + r * TURN + lane / CW];
+                if (e >= 0 && own < hi) static_cast<XT*>(a.out)[(long long)e * a.out_stride + own] = XT(y[h][r] + tile[(r * TURN + lane / CW) * CW + (lane & (CW - 1))]);
+              }
+              __syncwarp();
             }
           }
         } else if (a.out_f32) {
@@ -766,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
                   if (col + k < hi) o[col + k] = f[h] * acc[m][n][2 * h + k];
             }
           }
-        } else if (a.vec_out) {
+        } else if (a.by_out == kBy16) {
           // through the stage's room for rows, from where whole chunks leave
 #pragma unroll
           for (int h = 0; h < 2; h++)
@@ -829,7 +873,7 @@ cudaError_t launch_tile(const LoraArgs& a, int cluster, cudaStream_t st) {
 }
 template <typename XT, typename PT, bool BWD, int RT>
 cudaError_t launch_mt(const LoraArgs& a, int mt, int cluster, cudaStream_t st) {
-  if (a.by_in == kBy16 && a.by_w1 == kBy16 && a.by_w2 == kBy16)
+  if (a.by_in == kBy16 && a.by_w1 == kBy16 && a.by_w2 == kBy16 && (BWD || a.by_out == kBy16))
     return mt == 16 ? launch_tile<XT, PT, BWD, RT, 16, true>(a, cluster, st) : launch_tile<XT, PT, BWD, RT, 64, true>(a, cluster, st);
   return mt == 16 ? launch_tile<XT, PT, BWD, RT, 16, false>(a, cluster, st) : launch_tile<XT, PT, BWD, RT, 64, false>(a, cluster, st);
 }

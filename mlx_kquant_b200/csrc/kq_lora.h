@@ -63,7 +63,7 @@ struct LoraArgs {
   int direct;                 // tiles are found by the kernel itself: cluster c looks for the tile that entry c leads
   int n_clusters;             // tiles
   int by_in, by_w1, by_w2;    // how rows are read: by 16 bytes, 8, or elements
-  int vec_out;                // rows of base and out are whole aligned groups of 16 bytes
+  int by_out;                 // rows of base and out likewise
 };
 enum LoraTypes { kLoraBf16 = 0, kLoraF16 = 1, kLoraBf16F32 = 2, kLoraF16F32 = 3 };  // rows, and parameters where they are float32
 cudaError_t launch_lora_tile_bf16(const LoraArgs& a, bool backward, int mt, int cluster, cudaStream_t st);
@@ -109,7 +109,7 @@ struct LoraCall {
 cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_stride, void* out, long long out_stride, void* u,
                                 cudaStream_t st);
 size_t lora_saved_bytes(long long n, int r, int param_f32);
-size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int r, int param_f32);
+size_t lora_backward_workspace_bytes(long long n, int slots, int shared, int K, int N, int r, int param_f32);
 cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy_stride, const void* u, void* dx, long long dx_stride,
                                  void* da, void* db, void* workspace, cudaStream_t st);
 

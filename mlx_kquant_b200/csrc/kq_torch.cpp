@@ -190,7 +190,7 @@ struct LoraFunction : torch::autograd::Function<LoraFunction> {
     if (ctx->needs_input_grad(2)) out[2] = at::empty_like(a);
     if (ctx->needs_input_grad(3)) out[3] = at::empty_like(b);
     if (!out[1].defined() && !out[2].defined() && !out[3].defined()) return out;
-    const at::Tensor ws = bytes_of(std::max<size_t>(256, lora_backward_workspace_bytes(call.rows, call.slots, call.shared, call.K, call.rank, call.param)), x);
+    const at::Tensor ws = bytes_of(std::max<size_t>(256, lora_backward_workspace_bytes(call.rows, call.slots, call.shared, call.K, call.N, call.rank, call.param)), x);
     const int rc = lora_backward(dy.data_ptr(), call.type, call.rows, call.N, call.N, x.data_ptr(), call.K, call.K, call.slots, call.shared, a.data_ptr(),
                                  b.data_ptr(), call.param, call.rank, call.G, call.E, call.id(), call.expert(), call.factor(), call.scale, saved.data_ptr(),
                                  data(out[1]), data(out[2]), data(out[3]), data(plan), plan.defined() ? plan.numel() : 0, ws.data_ptr(), ws.numel(),

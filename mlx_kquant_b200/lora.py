@@ -81,7 +81,7 @@ class _Call:
         da = torch.empty_like(a) if need_a else None
         db = torch.empty_like(b) if need_b else None
         L = _lib.lib()
-        ws = torch.empty(max(256, L.kq_lora_backward_workspace_bytes(rows, self.slots, int(self.shared), K, r, _DT[a.dtype])),
+        ws = torch.empty(max(256, L.kq_lora_backward_workspace_bytes(rows, self.slots, int(self.shared), K, b.shape[-2], r, _DT[a.dtype])),
                          dtype=torch.uint8, device=dev)
         with _on_device(dev):
             check(L.kq_lora_backward(

@@ -77,7 +77,7 @@ def test_c_entries_refuse_before_touching_memory():
     need = L.kq_lora_plan_bytes(1000, 8)
     assert need > 1000 * 4 and L.kq_lora_plan_bytes(-1, 8) == 0 and L.kq_lora_plan_bytes(10, 0) == 0
     assert L.kq_lora_plan(p, None, 1000, 1, 8, 1, p, need - 1, None) == bad
-    assert L.kq_lora_backward_workspace_bytes(64, 1, 0, 4096, 16, F16) >= L.kq_lora_saved_bytes(64, 16, F16) == 64 * 16 * 4
+    assert L.kq_lora_backward_workspace_bytes(64, 1, 0, 4096, 4096, 16, F16) >= L.kq_lora_saved_bytes(64, 16, F16) == 64 * 16 * 4
     back = lambda ids=p, plan=None, ws=0: L.kq_lora_backward(  # noqa: E731
         p, F16, 4, 8, 8, p, 8, 8, 1, 0, p, p, F16, 2, 2, 1, ids, None, None, 1.0, p, p, p, p, plan, 1 << 20, p, ws, None)
     assert back() == bad and b"plan" in L.kq_last_error()
