@@ -309,7 +309,7 @@ def test_order_by_groups(n, slots, G, E):
         assert np.array_equal(order, np.argsort(key, kind="stable"))
         offsets = got[up(4 * n):up(4 * n) + 4 * (NG + 2)].view(np.int32)
         assert np.array_equal(offsets, np.concatenate([[0], np.cumsum(np.bincount(key, minlength=NG + 1))]))
-        height = 64 if n >= 24 * NG else 16
+        height = 64 if n > 2048 and n >= 24 * NG else 16
         at = up(up(4 * n) + 4 * (NG + 2))
         tiles = got[at:at + 16 * (n // height + NG + 1)].view(np.int32).reshape(-1, 4)
         seen = np.zeros(n, int)
