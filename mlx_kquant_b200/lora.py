@@ -30,6 +30,19 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return r if r.stride(1) == 1 or r.shape[1] == 1 and r.is_contiguous() else r.contiguous()
 
 
+def _integers(t: torch.Tensor) -> bool:
+    return t.dtype in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8, torch.uint16, torch.uint32)
+
+
+def _overlap(t: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether the bytes from t's first to its last meet the contiguous out's."""
+    if t.numel() == 0 or out.numel() == 0:
+        return False
+    t0, o0 = t.data_ptr(), out.data_ptr()
+    t1 = t0 + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return t0 < o0 + out.numel() * out.element_size() and o0 < t1
+
+
 def _i32(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype == torch.int64:   # (not wrapped around: what is out of range stays out of range)
         t = t.clamp(-1, 2 ** 31 - 1)
@@ -134,6 +147,20 @@ class _Update(torch.autograd.Function):
         return None, dy if need_y else None, dx, da, db
 
 
+class _Empty(torch.autograd.Function):
+    """A batch without rows: nothing to launch, gradients of zeros."""
+
+    @staticmethod
+    def forward(ctx, y, *others):
+        ctx.save_for_backward(y, *others)
+        return y.clone()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return tuple(torch.zeros_like(t) if need else None for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad))
+
+
 def _update(op, y, x, a, b, call, scaling, out, stream):
     """The checks that both forms share, and the call."""
     dev = x.device
@@ -171,8 +198,11 @@ def _update(op, y, x, a, b, call, scaling, out, stream):
             raise ValueError(f"[mlx_kquant.{op}] out= takes no part in gradients; leave it away.")
         if out.shape != y.shape or out.dtype != y.dtype or out.device != dev or not out.is_contiguous():
             raise ValueError(f"[mlx_kquant.{op}] out must be contiguous, of y's shape, dtype and device.")
+        itself = out.data_ptr() == y.data_ptr() and y.is_contiguous()
+        if any(_overlap(t, out) for t in ((x, a, b) if itself else (y, x, a, b))):
+            raise ValueError(f"[mlx_kquant.{op}] out must not overlap x, a, b or, unless it is y, y.")
     if y.numel() == 0:
-        return y.clone() if out is None else out
+        return _Empty.apply(y, x, a, b) if grads else y.clone() if out is None else out
     if grads:
         if stream is not None:
             raise ValueError(f"[mlx_kquant.{op}] stream= takes no part in gradients; set the current stream instead.")
@@ -193,7 +223,7 @@ def lora_update(y, x, a, b, adapter_ids=None, scaling=None, *, out=None, stream=
     for all rows below); outside [0, G): no adapter, the row stays y's. None: adapter 0 for every row. scaling: a number, or
     a tensor [G]; None: 1.
 
-    Returns a tensor like y, or writes to `out`, which may be y. Differentiable in y, x, a and b (not with `out` or `stream`). The
+    Returns a tensor like y, or writes to `out`, which may be y but overlaps nothing else. Differentiable in y, x, a and b (not with `out` or `stream`). The
     same call gives the same bits. A training step can be captured into a CUDA graph; as for every operator of torch, no eager
     autograd graph of the same leaves may be alive then."""
     if out is None and stream is None:
@@ -212,7 +242,7 @@ def lora_update(y, x, a, b, adapter_ids=None, scaling=None, *, out=None, stream=
     call.shared, call.n_experts, call.experts, call.ids, call.slots = False, 1, None, None, 1
     if adapter_ids is not None:
         lead = adapter_ids.dim()
-        if adapter_ids.shape != x.shape[:-1][:lead] or adapter_ids.is_floating_point() or adapter_ids.dtype == torch.bool:
+        if adapter_ids.shape != x.shape[:-1][:lead] or not _integers(adapter_ids):
             raise ValueError(f"[mlx_kquant.{op}] adapter_ids must be integers of x's leading axes {tuple(x.shape[:-1])} but got "
                              f"{adapter_ids.dtype} {tuple(adapter_ids.shape)}.")
         call.ids = _i32(adapter_ids, x.device)

@@ -955,7 +955,7 @@ def gather_lora_update(y, x, a, b, indices, adapter_ids=None, scaling=None, *, o
     [T, R, K], one per slot; a [G, E, r, K] and b [G, E, N, r] (without the first axis: one adapter for all); indices [T, R];
     adapter_ids [T], None: adapter 0. A slot whose expert is outside [0, E) or whose adapter is outside [0, G) stays y's. The rest is
     as in `lora_update`."""
-    from .lora import _Call, _i32, _update, front_update
+    from .lora import _Call, _i32, _integers, _update, front_update
 
     if out is None and stream is None and isinstance(indices, torch.Tensor):
         done = front_update(y, x, a, b, adapter_ids, scaling, indices)
@@ -971,14 +971,14 @@ def gather_lora_update(y, x, a, b, indices, adapter_ids=None, scaling=None, *, o
         raise ValueError(f"[mlx_kquant.{op}] y must be [T, R, N] and indices [T, R] but got {tuple(y.shape)}, {tuple(indices.shape)}.")
     if x.dim() not in (2, 3) or x.shape[:-1] != indices.shape[:x.dim() - 1]:
         raise ValueError(f"[mlx_kquant.{op}] x must be [T, K] or [T, R, K] but got {tuple(x.shape)} for indices {tuple(indices.shape)}.")
-    if indices.is_floating_point() or indices.dtype == torch.bool:
+    if not _integers(indices):
         raise ValueError(f"[mlx_kquant.{op}] indices must be integers but are {indices.dtype}.")
     call = _Call()
     call.shared, call.n_experts, call.slots, call.ids = x.dim() == 2, a.shape[1], max(1, indices.shape[1]), None
     if a.shape[0] * a.shape[1] > 65535:
         raise ValueError(f"[mlx_kquant.{op}] needs adapters * experts <= 65535.")
     if adapter_ids is not None:
-        if adapter_ids.shape != indices.shape[:1] or adapter_ids.is_floating_point() or adapter_ids.dtype == torch.bool:
+        if adapter_ids.shape != indices.shape[:1] or not _integers(adapter_ids):
             raise ValueError(f"[mlx_kquant.{op}] adapter_ids must be integers of shape ({indices.shape[0]},) but got "
                              f"{adapter_ids.dtype} {tuple(adapter_ids.shape)}.")
         call.ids = _i32(adapter_ids, x.device)

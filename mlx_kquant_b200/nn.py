@@ -254,7 +254,7 @@ class KQuantLoRASwitchLinear(torch.nn.Module):
         slots = indices.reshape(-1, 1) if flat else indices
         T, R = slots.shape
         rows = x.reshape(T, R, K) if flat or x.shape[1] == R else x.reshape(T, K)
-        return gather_lora_update(y.reshape(T, R, -1), rows, self.lora_a, self.lora_b, slots, adapter_ids, self.scaling).reshape(y.shape)
+        return gather_lora_update(y.reshape(T, R, y.shape[-1]), rows, self.lora_a, self.lora_b, slots, adapter_ids, self.scaling).reshape(y.shape)
 
     def extra_repr(self) -> str:
         n, e, r, _ = self.lora_a.shape
