@@ -346,7 +346,7 @@ KQ_API int kq_gather_qmm_seg(const void* x, int x_dtype, long long rows, int K, 
  *   = scale * s / (sum of the picked s + 1e-20), or scale * s without norm_topk_prob; indices int32 [T, top_k].
  *   An expert whose logit (or bias) is -infinity is not available; where fewer than top_k are, the rest of the row is index -1 with
  *   weight 0, which the expert products skip. A NaN logit is picked first and makes the row's weights NaN (with sigmoid and
- *   without norm_topk_prob its own alone). E <= 1024, top_k <= 32, E a multiple of n_groups.
+ *   without norm_topk_prob its own alone). T <= 2^30, E <= 1024, top_k <= 32, E a multiple of n_groups.
  * kq_moe_router_grouped_backward: dlogits [T, E] of `dtype` from dweights float32 [T, top_k], for the same logits and the indices
  *   that the call above gave (the bias and the groups only choose: they have no gradient). */
 KQ_API int kq_moe_router_grouped(const void* logits, int dtype, long long T, int E, int top_k, int n_groups, int top_groups,
@@ -374,7 +374,7 @@ KQ_API int kq_moe_router_grouped_backward(const void* logits, int dtype, long lo
  *    kq_lora_backward unless adapter_ids and experts are both NULL; kq_lora_update takes NULL too, but then looks for the rows of each
  *    group in every call: meant for up to 128 entries.
  *  workspace: kq_lora_backward_workspace_bytes(...) bytes, 256-byte aligned, private to the call until it completes.
- *  The same call gives the same bits. rows < 2^31, n_adapters * n_experts <= 65535. */
+ *  The same call gives the same bits. rows, K, N <= 2^30, n_adapters * n_experts <= 65535. */
 KQ_API size_t kq_lora_plan_bytes(long long rows, int n_groups);
 KQ_API int kq_lora_plan(const int32_t* adapter_ids, const uint32_t* experts, long long rows, int slots, int n_adapters,
                         int n_experts, void* plan, size_t plan_bytes, void* stream);

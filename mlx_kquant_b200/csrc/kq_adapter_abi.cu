@@ -1,5 +1,4 @@
 // The C entry points of the grouped router and of the low-rank adapters: argument checks, then the launches.
-#include <climits>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -27,6 +26,9 @@ int done(const char* what, cudaError_t e) {
   return e == cudaSuccess ? KQ_OK : fail(KQ_ERR_CUDA, "[mlx_kquant] %s: CUDA error: %s", what, cudaGetErrorString(e));
 }
 
+// rows, and values of a row: the kernels count them in 32 bits, some steps ahead of the last
+constexpr int kMost = 1 << 30;
+
 int route_check(const char* op, int dtype, long long T, int E, int top_k, const char* scoring, int* code) {
   if (scoring != nullptr && std::strcmp(scoring, "softmax") == 0) *code = 0;
   else if (scoring == nullptr || std::strcmp(scoring, "sigmoid") == 0) *code = 1;
@@ -35,7 +37,7 @@ int route_check(const char* op, int dtype, long long T, int E, int top_k, const 
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] logits must be floating.", op);
   if (E < 1 || E > 1024 || top_k < 1 || top_k > 32 || top_k > E)
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] needs 1 <= top_k <= min(E, 32) and E <= 1024.", op);
-  if (T < 0 || T > INT_MAX) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] bad token count.", op);
+  if (T < 0 || T > kMost) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] bad token count.", op);
   return KQ_OK;
 }
 
@@ -44,10 +46,10 @@ int lora_check(const char* op, int dtype, int param_dtype, long long rows, int K
                int n_experts, const void* adapter_ids, const void* experts, const void* plan, size_t plan_bytes) {
   if ((dtype != KQ_F16 && dtype != KQ_BF16) || (param_dtype != dtype && param_dtype != KQ_F32))
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] rows must be float16 or bfloat16, parameters of the same type or float32.", op);
-  if (K < 1 || N < 1 || K > INT_MAX - 64 || N > INT_MAX - 64) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] bad row length.", op);
+  if (K < 1 || N < 1 || K > kMost || N > kMost) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] bad row length.", op);
   if (rank < 1 || rank > kq::kLoraMaxRank)
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] rank must be 1 to %d but is %d.", op, kq::kLoraMaxRank, rank);
-  if (rows < 0 || rows > INT_MAX - 64 || slots < 1 || rows % slots != 0)
+  if (rows < 0 || rows > kMost || slots < 1 || rows % slots != 0)
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] bad row count.", op);
   if (n_adapters < 1 || n_experts < 1 || (long long)n_adapters * n_experts > 65535)
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] needs 1 <= adapters * experts <= 65535.", op);
@@ -120,7 +122,7 @@ int kq_moe_router_grouped_backward(const void* logits, int dtype, long long T, i
 }
 
 size_t kq_lora_plan_bytes(long long rows, int n_groups) {
-  return rows < 0 || rows > INT_MAX - 64 || n_groups < 1 || n_groups > 65535 ? 0 : kq::lora_plan_layout(rows, n_groups).total;
+  return rows < 0 || rows > kMost || n_groups < 1 || n_groups > 65535 ? 0 : kq::lora_plan_layout(rows, n_groups).total;
 }
 
 int kq_lora_plan(const int32_t* adapter_ids, const uint32_t* experts, long long rows, int slots, int n_adapters, int n_experts,

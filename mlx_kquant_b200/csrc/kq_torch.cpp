@@ -264,7 +264,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (a.dim() != d || b.dim() != d || x.dim() < 1 || y.dim() < 1) Py_RETURN_NONE;
   const int64_t G = a.size(0), E = gathered ? a.size(1) : 1, r = a.size(-2), K = a.size(-1), N = b.size(-2);
   if (b.size(0) != G || (gathered && b.size(1) != E) || b.size(-1) != r || x.size(-1) != K || y.size(-1) != N || r < 1 || r > 128 ||
-      K > INT32_MAX - 64 || N > INT32_MAX - 64 || G * E > 65535)
+      K > 1 << 30 || N > 1 << 30 || G * E > 65535)
     Py_RETURN_NONE;
   const int64_t rows = y.numel() / N;
   int64_t slots = 1;
@@ -309,7 +309,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const int64_t direct = PyLong_AsLongLong(args[7]);
   if (PyErr_Occurred()) return nullptr;
-  if (rows > INT32_MAX - 64) Py_RETURN_NONE;
+  if (rows > 1 << 30) Py_RETURN_NONE;
   const Lora call{type, param, (int)K, (int)N, (int)r, (int)G, (int)E, (int)slots, rows, shared, ids, experts, scaling, (float)scale};
   if (wants_gradient(y) || wants_gradient(x) || wants_gradient(a) || wants_gradient(b))
     return THPVariable_Wrap(LoraFunction::apply(y, x, a, b, call));
