@@ -538,6 +538,11 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
           if (FAST || a.by_out == kBy16) cp16_sized(to, row + (there ? c : 0), there ? 16 : 0);
           else load_chunk<2>(to, row, c, there ? hi - lo : 0, kBy8);
         }
+      } else if (!BWD && tid < MT && s_row[tid] >= 0 && c0 < hi - lo) {
+        // rows that start anywhere are read by column when the stage is multiplied: from L2 then
+        const XT* p = static_cast<const XT*>(a.base) + (long long)s_row[tid] * a.base_stride + lo + c0;
+        const uintptr_t from = reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15, to = (reinterpret_cast<uintptr_t>(p + min(NB, hi - lo - c0)) + 15) & ~(uintptr_t)15;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(__cvta_generic_to_global(reinterpret_cast<const void*>(from))), "r"((uint32_t)(to - from)) : "memory");
       }
     }
     next++;
@@ -709,6 +714,24 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
     fetch();
     const int c0 = lo + s * NB;
     if (m0 < t.rows && c0 + cw < hi) {
+      // forward, rows that start anywhere: eight rows at a time, a column a lane, so that an access is a run of a row; all at once, and
+      // what lies outside is read from the tile's first row or the last column instead
+      constexpr int TURN = 32 / CW;   // rows at once
+      const bool anywhere = !BWD && !FAST && a.by_out == kByElement;
+      const int own = c0 + cw + (lane & (CW - 1));
+      uint16_t y[MW][2][8 / TURN];
+      if (anywhere) {
+        const uint16_t* p = static_cast<const uint16_t*>(a.base) + min(own, hi - 1);
+#pragma unroll
+        for (int m = 0; m < MW; m++)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 8 / TURN; r++) {
+              const int e = s_row[m0 + 16 * m + 8 * h + r * TURN + lane / CW];
+              y[m][h][r] = p[(long long)(e < 0 ? s_row[0] : e) * a.base_stride];
+            }
+      }
       float acc[MW][CW / 8][4];
 #pragma unroll
       for (int m = 0; m < MW; m++)
@@ -768,20 +791,9 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
               }
             }
           } else {
-            // Rows that start anywhere: through shared memory in float32, eight rows at a time, to a column a lane, so that an access
-            // is a run of a row.
-            const int own = c0 + cw + (lane & (CW - 1));
-            constexpr int TURN = 32 / CW;   // rows at once
+            // through shared memory in float32
             float* tile = reinterpret_cast<float*>(smem + (at - ring)) + warp * 8 * CW;
             static_assert(kThreads / 32 * 8 * CW * 4 <= S::Y, "the stage's room for rows");
-            float y[2][8 / TURN];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-              for (int r = 0; r < 8 / TURN; r++) {
-                const int e = s_row[m0 + 16 * m + 8 * h + r * TURN + lane / CW];
-                y[h][r] = e >= 0 && own < hi ? to_float(static_cast<const XT*>(a.base)[(long long)e * a.base_stride + own]) : 0.f;
-              }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
 #pragma unroll
@@ -790,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
 #pragma unroll
               for (int r = 0; r < 8 / TURN; r++) {
                 const int e = s_row[m0 + 16 * m + 8 * h + r * TURN + lane / CW];
-                if (e >= 0 && own < hi) static_cast<XT*>(a.out)[(long long)e * a.out_stride + own] = XT(y[h][r] + tile[(r * TURN + lane / CW) * CW + (lane & (CW - 1))]);
+                if (e >= 0 && own < hi) static_cast<XT*>(a.out)[(long long)e * a.out_stride + own] = XT(to_float(*reinterpret_cast<const XT*>(&y[m][h][r])) + tile[(r * TURN + lane / CW) * CW + (lane & (CW - 1))]);
               }
               __syncwarp();
             }
