@@ -498,12 +498,17 @@ int sm_count() {
   return sms;
 }
 
-// CTAs of a cluster: as many as fill the GPU twice at most
-int pick_cluster(long long tiles) {
-  const long long room = 2LL * sm_count();
-  for (int c = 8; c > 1; c >>= 1)
-    if (tiles * c <= room) return c;
-  return 1;
+// CTAs of a cluster, for that many tiles and as many CTAs as an SM holds: what fills the GPU but still runs at once. Clusters
+// stay within a group of SMs, so larger ones leave a few of them empty: a tenth is kept back. Rows in tiles of 64, K 1024, N 2048, rank
+// 16, clusters of 2, 3, 4, 6, 8: 30 tiles 15.0, 13.2, 12.5, 12.8, 11.8 us; 40 tiles 15.2, 13.3, 14.3, 13.0, 20.5; 60 tiles 15.5, 17.5,
+// 14.4, 23.4, 21.2; 72 tiles 15.7, 17.6, 23.0 (no longer at once); 80 tiles 21.0, 17.7, 23.3; 96 tiles 21.6, 28.0.
+int pick_cluster(long long tiles, int per_sm) {
+  const long long sms = sm_count(), room = per_sm * sms;
+  auto fits = [&](int c) { return 10 * tiles * c <= 9 * room; };
+  for (int c : {8, 6, 4})
+    if (fits(c)) return c;
+  if (per_sm > 1 && 2 * tiles <= sms) return 2;   // an SM for each CTA
+  return fits(3) ? 3 : 2 * tiles <= room ? 2 : 1;
 }
 
 constexpr size_t kSlotBytes = 64u << 20;          // float32 rows of slots that are summed at a time: they stay in L2
@@ -542,7 +547,8 @@ int set_rows(LoraArgs& a, const LoraCall& c, int& cluster) {
   // tiles that have rows, as far as the host knows: those found one by one are no more than the groups; half of the groups' last
   // tiles of a plan are counted (4072 entries of 128 groups: clusters of 1, 2, 4, 8 forward 47, 30, 37, 56 us)
   const long long groups = (long long)c.g.G * c.g.E;
-  cluster = pick_cluster(a.direct ? std::min(c.g.n, groups) : grouped ? c.g.n / mt + std::min(c.g.n, groups) / 2 : a.n_clusters);
+  cluster = pick_cluster(a.direct ? std::min(c.g.n, groups) : grouped ? c.g.n / mt + std::min(c.g.n, groups) / 2 : a.n_clusters,
+                         a.r > 64 ? 1 : 2);
   return mt;
 }
 
@@ -733,7 +739,7 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
   w.tiles = (w.of[0].D + 127) / 128;
   // CTAs of a cluster share a group's stages of 64 entries, where the columns alone leave the GPU empty
   const long long stages = (c.g.n / w.n_groups + 63) / 64, all = w.tiles + (n > 1 ? (w.of[1].D + 127) / 128 : 0);
-  cluster = pick_cluster(w.n_groups * all);
+  cluster = pick_cluster(w.n_groups * all, a.r > 32 ? 1 : 2);
   while (cluster > 1 && stages < 2 * cluster) cluster >>= 1;
   return launch_lora_wgrad(w, f16 ? 1 : 2, f32, cluster, st);
 }
