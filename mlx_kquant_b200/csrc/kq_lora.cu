@@ -502,12 +502,13 @@ int sm_count() {
 // stay within a group of SMs, so larger ones leave a few of them empty: a tenth is kept back. Rows in tiles of 64, K 1024, N 2048, rank
 // 16, clusters of 2, 3, 4, 6, 8: 30 tiles 15.0, 13.2, 12.5, 12.8, 11.8 us; 40 tiles 15.2, 13.3, 14.3, 13.0, 20.5; 60 tiles 15.5, 17.5,
 // 14.4, 23.4, 21.2; 72 tiles 15.7, 17.6, 23.0 (no longer at once); 80 tiles 21.0, 17.7, 23.3; 96 tiles 21.6, 28.0.
-int pick_cluster(long long tiles, int per_sm) {
+// `exact`: no other CTAs are in the grid (those of a plan's empty slots take SMs for a moment, and two CTAs then share one).
+int pick_cluster(long long tiles, int per_sm, bool exact) {
   const long long sms = sm_count(), room = per_sm * sms;
   auto fits = [&](int c) { return 10 * tiles * c <= 9 * room; };
   for (int c : {8, 6, 4})
     if (fits(c)) return c;
-  if (per_sm > 1 && 2 * tiles <= sms) return 2;   // an SM for each CTA
+  if (per_sm > 1 && exact && 2 * tiles <= sms) return 2;   // an SM for each CTA
   return fits(3) ? 3 : 2 * tiles <= room ? 2 : 1;
 }
 
@@ -530,7 +531,10 @@ int set_rows(LoraArgs& a, const LoraCall& c, int& cluster) {
   const bool grouped = c.g.ids != nullptr || c.g.experts != nullptr;
   int mt;
   if (!grouped) {
-    mt = c.g.n <= 1280 ? 16 : 64;   // (600 rows, K, N 4096, rank 16: 9.9 and 12.7 us; 1200 14.9 and 15.7)
+    // Low tiles while two CTAs of each run at once, and the matrices that each tile reads are small. K, N 4096, rank 16: 1300 rows 12.9 and
+    // 16.0 us in tiles of 16 and 64, 2368 rows 16.0 and 19.8, 2700 rows 23.2 and 20.6; float32 1300 rows 18.4 and 20.5, 1700 24.1 and 20.6.
+    const long long matrices = (long long)c.r * ((long long)c.K + c.N) * (c.types == kLoraBf16 || c.types == kLoraF16 ? 2 : 4);
+    mt = c.g.n <= (matrices < (512 << 10) ? 16 * sm_count() : 1280) ? 16 : 64;
     a.n_clusters = (int)((c.g.n + mt - 1) / mt);
   } else if (c.plan != nullptr) {
     const LoraPlanLayout l = lora_plan_layout(c.g.n, c.g.G * c.g.E);
@@ -548,7 +552,7 @@ int set_rows(LoraArgs& a, const LoraCall& c, int& cluster) {
   // tiles of a plan are counted (4072 entries of 128 groups: clusters of 1, 2, 4, 8 forward 47, 30, 37, 56 us)
   const long long groups = (long long)c.g.G * c.g.E;
   cluster = pick_cluster(a.direct ? std::min(c.g.n, groups) : grouped ? c.g.n / mt + std::min(c.g.n, groups) / 2 : a.n_clusters,
-                         a.r > 64 ? 1 : 2);
+                         a.r > 64 ? 1 : 2, !grouped);
   return mt;
 }
 
@@ -739,7 +743,7 @@ cudaError_t launch_lora_backward(const LoraCall& c, const void* dy, long long dy
   w.tiles = (w.of[0].D + 127) / 128;
   // CTAs of a cluster share a group's stages of 64 entries, where the columns alone leave the GPU empty
   const long long stages = (c.g.n / w.n_groups + 63) / 64, all = w.tiles + (n > 1 ? (w.of[1].D + 127) / 128 : 0);
-  cluster = pick_cluster(w.n_groups * all, a.r > 32 ? 1 : 2);
+  cluster = pick_cluster(w.n_groups * all, a.r > 32 ? 1 : 2, true);
   while (cluster > 1 && stages < 2 * cluster) cluster >>= 1;
   return launch_lora_wgrad(w, f16 ? 1 : 2, f32, cluster, st);
 }
