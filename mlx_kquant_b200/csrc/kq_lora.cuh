@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
           if (FAST || a.by_out == kBy16) cp16_sized(to, row + (there ? c : 0), there ? 16 : 0);
           else load_chunk<2>(to, row, c, there ? hi - lo : 0, kBy8);
         }
-      } else if (!BWD && tid < MT && s_row[tid] >= 0 && c0 < hi - lo) {
+      } else if (!BWD && !FAST && tid < MT && s_row[tid] >= 0 && c0 < hi - lo) {
         // rows that start anywhere are read by column when the stage is multiplied: from L2 then
         const XT* p = static_cast<const XT*>(a.base) + (long long)s_row[tid] * a.base_stride + lo + c0;
         const uintptr_t from = reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15, to = (reinterpret_cast<uintptr_t>(p + min(NB, hi - lo - c0)) + 15) & ~(uintptr_t)15;
