@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
   const int blocks = a.shrink ? (a.D1 + KB - 1) / KB : 0;
   const int b0 = blocks * rank / C, n1 = blocks * (rank + 1) / C - b0;
   const int n2 = a.out != nullptr ? (hi - lo + NB - 1) / NB : 0;
-  const bool staged = a.base != nullptr && a.by_out != kByElement;   // the base's rows come with the weights
+  const bool staged = !BWD && (FAST || a.by_out != kByElement);   // the base's rows come with the weights
   const uint32_t ring = smem_at(smem);
 
   // This thread's chunks: where they come from in the first stage of each product, and where they go. A row or rank that does not
