@@ -345,11 +345,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
       }
     lo = -rt_max(-least);
     hi = rt_max(most) + 1.f;
+    if (a.G > 1 && a.group_top > 1) {   // the range holds zero too, which is what the second of a single available expert counts
+      lo = fminf(lo, 0.f);
+      hi = fmaxf(hi, 0.f);
+    }
     slack *= 1.f + fmaxf(fabsf(lo), fabsf(hi));
     odd = __any_sync(kAll, odd);
   }
-  // score + bias as fixed point: unit * s + shift, from 0 at the least bias
+  // score + bias as fixed point: unit * s + shift, from 0 at the least bias (or at zero); a code's upper bits are one more
   const float unit = UNITS / (hi - lo);
+  const uint32_t nothing = by_score ? (uint32_t)(-lo * unit) + 1u : 0u;   // a sum of two holds the range's offset twice, of one likewise then
   float shift[NI];
 #pragma unroll
   for (int i = 0; i < NI; i++) shift[i] = by_score ? (bias[i] - lo) * unit : 0.f;
@@ -429,7 +434,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
         for (int i = 0; i < NI; i++) merge_two(groups_by_score ? code[i] : by[i], 0, b0, b1);
         for (int o = 1; o < lanes; o <<= 1) merge_two(__shfl_xor_sync(kAll, b0, o), __shfl_xor_sync(kAll, b1, o), b0, b1);
         // lane g comes to have group g: what it counts, and its index counted down; none without an expert
-        const uint32_t count = __shfl_sync(kAll, a.group_top > 1 ? (b0 >> IB) + (b1 >> IB) : b0 >> IB, lane * lanes & 31);
+        const uint32_t second = b1 != 0 ? b1 >> IB : b0 != 0 ? nothing : 0u;
+        const uint32_t count = __shfl_sync(kAll, a.group_top > 1 ? (b0 >> IB) + second : b0 >> IB, lane * lanes & 31);
         const uint32_t whole = lane < a.G && count != 0 ? count << 5 | (31 - lane) : 0u;
         uint32_t mine = whole, last = 0;
         bool stays = false;
