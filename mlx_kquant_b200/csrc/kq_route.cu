@@ -547,7 +547,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps, route_ctas<NI>()) route_kern
   }
 }
 
-// dl from dw. A warp per token; everything but the picks is zero, except with softmax scores that are not renormalised.
+// dl from dw. A warp per token; everything but the picks is zero, except with softmax scores that are not renormalised (or whose picks'
+// sum is next to nothing).
 template <typename T, int NI>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(const RouteArgs a) {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;\n" ::: "memory");
@@ -579,16 +580,21 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(const 
     fz = rt_sum(z);
   }
   if (idx >= 0) s = a.scoring == 0 ? expf(x - fm) / fz : rt_sigmoid(x);
-  float ds = dw;
+  // softmax: every expert has -s times the picks' sum of ds s. Renormalised, that is dw's mean over the picks times 1e-20 / S: beside the
+  // row's other entries less than half a float's last bit, and left away, as long as S is above 1e-12.
+  float ds = dw, all = 0.f;
+  bool whole_row = a.scoring == 0;
   if (a.norm) {
-    const float S = rt_sum(s) + 1e-20f;
-    ds = (dw - rt_sum(dw * (s / S))) / S;
+    const float S = rt_sum(s) + 1e-20f, mean = rt_sum(dw * (s / S));
+    ds = (dw - mean) / S;
+    all = mean * (1e-20f / S);
+    whole_row = whole_row && S < 1e-12f;
   }
   const float dl = a.scoring == 1 ? ds * s * rt_sigmoid(-x) : ds * s;
+  if (!a.norm && whole_row) all = rt_sum(dl);
   float d[NI];
-  const float all = a.scoring == 0 && !a.norm ? rt_sum(dl) : 0.f;
 #pragma unroll
-  for (int i = 0; i < NI; i++) d[i] = a.scoring == 0 && !a.norm && l[i] != -INFINITY ? -(expf(l[i] - fm) / fz) * all : 0.f;
+  for (int i = 0; i < NI; i++) d[i] = whole_row && l[i] != -INFINITY ? -(expf(l[i] - fm) / fz) * all : 0.f;
   for (int r = 0; r < a.top_k; r++) {
     const int e = __shfl_sync(kAll, idx, r);
     const float v = __shfl_sync(kAll, dl, r);
