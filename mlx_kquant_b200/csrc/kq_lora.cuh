@@ -678,10 +678,11 @@ __global__ void __launch_bounds__(kThreads, Shape<PT, BWD, RT, MT>::CTAS) tile_k
     }
     float f = 1.f;
     if constexpr (std::is_same<CT, __half>::value) {
-      // fp16 terms: the largest of the row comes to lie in [1, 2)
+      // fp16 terms: the row's largest comes to lie in [2^14, 2^15), so that parts down to 2^-23 of it still have 16 bits in their two
+      // terms (fp16's steps end at 2^-24; the largest in [1, 2) left parts of 2^-20 with five)
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (most > 0.f && most < INFINITY) f = __uint_as_float(max(1u, min(253u, __float_as_uint(most) >> 23)) << 23);
+      if (most > 0.f && most < INFINITY) f = __uint_as_float((unsigned)max(1, (int)(__float_as_uint(most) >> 23) - 14) << 23);
     }
 #pragma unroll
     for (int b = 0; b < (RP + 31) / 32; b++) {
