@@ -279,7 +279,4 @@ def quantized_matmul_lora(x, w, scales, kquant_type, a, b, adapter_ids=None, sca
         y = _FrozenMatmul.apply(x, w, scales, kquant_type) if x.requires_grad else quantized_matmul(x, w, scales, kquant_type)
         return lora_update(y, x, a, b, adapter_ids, scaling)
     y = quantized_matmul(x, w, scales, kquant_type, stream=stream)
-    if stream is None:
-        return lora_update(y, x, a, b, adapter_ids, scaling, out=y)
-    with torch.cuda.stream(stream):   # y is this stream's already
-        return lora_update(y, x, a, b, adapter_ids, scaling, out=y)
+    return lora_update(y, x, a, b, adapter_ids, scaling, out=y, stream=stream)
