@@ -204,7 +204,7 @@ class KQuantLoRALinear(torch.nn.Module):
 
 
 class _FrozenGather(torch.autograd.Function):
-    """gather_qmm over an expert stack with the gradient of its rows; the wire bytes have none."""
+    """gather_qmm over an expert stack with the gradient of its rows; the wire bytes have none. All indices lie in the stack."""
 
     @staticmethod
     def forward(ctx, x, w, scales, kquant_type, indices):
@@ -217,16 +217,15 @@ class _FrozenGather(torch.autograd.Function):
     def backward(ctx, dy):
         w, indices = ctx.saved_tensors
         dx = kq.gather_qmm(dy, w, None, ctx.kquant_type, rhs_indices=indices, transpose=False)
-        there = (indices >= 0) & (indices < w.shape[0])   # rows of other entries are not written
-        dx = torch.where(there[..., None, None], dx.float(), 0.0)
-        return dx.sum_to_size(ctx.x_shape).to(ctx.dtype), None, None, None, None
+        return dx.float().sum_to_size(ctx.x_shape).to(ctx.dtype), None, None, None, None
 
 
 class KQuantLoRASwitchLinear(torch.nn.Module):
     """Low-rank adapters on a `KQuantSwitchLinear`: a pair of matrices for every adapter and expert, `lora_a` [n_adapters, n_experts,
     rank, in_dims], `lora_b` [n_adapters, n_experts, out_dims, rank]. `forward(x, indices, adapter_ids, sorted_indices)` takes what the
     base takes for routed rows: indices [T, R] with x [T, 1, 1, K] (one row per token) or [T, R, 1, K] and adapter_ids [T], or
-    indices [B] with x [B, 1, K] and adapter_ids [B] (`moe.gather_lora_update`)."""
+    indices [B] with x [B, 1, K] and adapter_ids [B] (`moe.gather_lora_update`). Rows of an index outside the stack, as the router's
+    -1, are zero, without bias."""
 
     def __init__(self, base: KQuantSwitchLinear, rank: int, n_adapters: int = 1, scaling: float = 1.0,
                  dtype: torch.dtype = torch.float32):
@@ -247,10 +246,14 @@ class KQuantLoRASwitchLinear(torch.nn.Module):
                              and x.shape[1] in (1, indices.shape[1])):
             raise ValueError(f"KQuantLoRASwitchLinear: x must be [T, 1, 1, K] or [T, R, 1, K] with indices [T, R], or [B, 1, K] with "
                              f"indices [B], but x is {tuple(x.shape)} and indices {tuple(indices.shape)}.")
+        # the base's product leaves rows of other indices unwritten and looks for their bias: they take an expert's place and become zero
+        whole = indices.to(base.weight.device, indices.dtype if indices.dtype in (torch.int32, torch.int64) else torch.int64)
+        near = whole.clamp(0, base.weight.shape[0] - 1)   # (in order where the indices are)
         if torch.is_grad_enabled() and x.requires_grad:
-            y = base._add_bias(_FrozenGather.apply(x, base.weight, base.scales, base.kquant_type, indices), indices)
+            y = base._add_bias(_FrozenGather.apply(x, base.weight, base.scales, base.kquant_type, near), near)
         else:
-            y = base(x, indices, sorted_indices)
+            y = base(x, near, sorted_indices)
+        y = torch.where((near == whole)[..., None, None], y, 0.0)
         slots = indices.reshape(-1, 1) if flat else indices
         T, R = slots.shape
         rows = x.reshape(T, R, K) if flat or x.shape[1] == R else x.reshape(T, K)
