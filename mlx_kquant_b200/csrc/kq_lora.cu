@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && SHORT ? 4 : RT <= 2 ? 2 :
     __syncthreads();
   }
   if (C > 1) cluster.sync();
-  const float f = a.scaled ? factor_of(both.g, group) : 1.f;
+  const float f = a.scaled && count > 0 ? factor_of(both.g, group) : 1.f;   // (zero times a factor may be NaN)
   const int r1 = min(RP, both.r - j0), cols = min(S::COLS, a.D - c0);
   PT* out = static_cast<PT*>(a.out) + (long long)group * both.r * a.D;
   // rows of the gradient's tile: ranks (r_first) or columns; four neighbours a thread
