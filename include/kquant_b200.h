@@ -368,7 +368,7 @@ KQ_API int kq_moe_router_grouped_backward(const void* logits, int dtype, long lo
  *    where x_shared; da and db, of the parameters' type and shape, whole (zero for groups without entries). Each may be NULL. What
  *    flows to y is dy itself.
  *  dtype: of x, y, out, dy, dx: KQ_F16 or KQ_BF16; param_dtype: of a, b, da, db: the same, or KQ_F32. rank <= 128. Row strides in
- *    elements, rows dense. Any K, N, rank and alignment; whole groups of 16 bytes are faster.
+ *    elements, rows dense. Any K, N, rank, and alignment to an element's size; whole groups of 16 bytes are faster.
  *  plan: the entries in the order of their groups, made by kq_lora_plan in kq_lora_plan_bytes(rows, n_adapters * n_experts)
  *    bytes of device memory (256-byte aligned) for the same adapter_ids, experts, rows, slots, n_adapters, n_experts. Needed by
  *    kq_lora_backward unless adapter_ids and experts are both NULL; kq_lora_update takes NULL too, but then looks for the rows of each

@@ -2,6 +2,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/kquant_b200.h"
 #include "kq_lora.h"
@@ -28,6 +29,19 @@ int done(const char* what, cudaError_t e) {
 
 // rows, and values of a row: the kernels count them in 32 bits, some steps ahead of the last
 constexpr int kMost = 1 << 30;
+
+struct Operand {
+  const char* name;
+  const void* p;
+  int align;
+};
+int aligned_check(const char* op, std::initializer_list<Operand> all) {
+  for (const Operand& o : all)
+    if (reinterpret_cast<uintptr_t>(o.p) % o.align != 0)
+      return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] %s must be %d-byte aligned.", op, o.name, o.align);
+  return KQ_OK;
+}
+int size_of(int dtype) { return dtype == KQ_F32 ? 4 : 2; }
 
 int route_check(const char* op, int dtype, long long T, int E, int top_k, const char* scoring, int* code) {
   if (scoring != nullptr && std::strcmp(scoring, "softmax") == 0) *code = 0;
@@ -85,6 +99,7 @@ int kq_moe_router_grouped(const void* logits, int dtype, long long T, int E, int
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] the kept groups have fewer than top_k experts.", op);
   if (T == 0) return KQ_OK;
   if (!logits || !indices || !weights) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] null pointer.", op);
+  if (int off = aligned_check(op, {{"logits", logits, size_of(dtype)}, {"bias", bias, 4}, {"indices", indices, 4}, {"weights", weights, 4}})) return off;
   a.logits = logits;
   a.dtype = dtype;
   a.T = (int)T;
@@ -108,6 +123,8 @@ int kq_moe_router_grouped_backward(const void* logits, int dtype, long long T, i
   const int rc = route_check(op, dtype, T, E, top_k, scoring, &a.scoring);
   if (rc != KQ_OK || T == 0) return rc;
   if (!logits || !indices || !dweights || !dlogits) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] null pointer.", op);
+  if (int off = aligned_check(op, {{"logits", logits, size_of(dtype)}, {"indices", indices, 4}, {"dweights", dweights, 4}, {"dlogits", dlogits, size_of(dtype)}}))
+    return off;
   a.logits = logits;
   a.dtype = dtype;
   a.T = (int)T;
@@ -133,6 +150,7 @@ int kq_lora_plan(const int32_t* adapter_ids, const uint32_t* experts, long long 
   if (plan == nullptr || plan_bytes < kq_lora_plan_bytes(rows, n_adapters * n_experts))
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] the plan is smaller than kq_lora_plan_bytes.", op);
   if (adapter_ids == nullptr && experts == nullptr) return KQ_OK;
+  if (int off = aligned_check(op, {{"the plan", plan, 256}, {"adapter_ids", adapter_ids, 4}, {"experts", experts, 4}})) return off;
   return done(op, kq::launch_lora_plan(kq::LoraGroups{adapter_ids, experts, slots, n_adapters, n_experts, rows, nullptr, 1.f}, plan,
                                        static_cast<cudaStream_t>(stream)));
 }
@@ -145,6 +163,9 @@ int kq_lora_update(const void* x, int dtype, long long rows, int K, long long x_
   const int rc = lora_check(op, dtype, param_dtype, rows, K, N, rank, slots, n_adapters, n_experts, adapter_ids, experts, plan, plan_bytes);
   if (rc != KQ_OK || rows == 0) return rc;
   if (!x || !a || !b || !y || !out) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] null pointer.", op);
+  if (int off = aligned_check(op, {{"x", x, 2}, {"a", a, size_of(param_dtype)}, {"b", b, size_of(param_dtype)}, {"y", y, 2}, {"out", out, 2}, {"saved", u, 16},
+                                   {"adapter_ids", adapter_ids, 4}, {"experts", experts, 4}, {"scaling", scaling, 4}, {"the plan", plan, 256}}))
+    return off;
   const kq::LoraCall c{types_of(dtype, param_dtype), kq::LoraGroups{adapter_ids, experts, slots, n_adapters, n_experts, rows, scaling, scale},
                        x, x_row_stride, x_shared, K, N, rank, a, b, plan};
   return done(op, kq::launch_lora_forward(c, y, y_row_stride, out, out_row_stride, u, static_cast<cudaStream_t>(stream)));
@@ -180,6 +201,10 @@ int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] needs the plan of its indices.", op);
   if (workspace == nullptr || workspace_bytes < kq_lora_backward_workspace_bytes(rows, slots, x_shared, K, N, rank, param_dtype))
     return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] workspace is smaller than kq_lora_backward_workspace_bytes.", op);
+  if (int off = aligned_check(op, {{"dy", dy, 2}, {"x", x, 2}, {"a", a, size_of(param_dtype)}, {"b", b, size_of(param_dtype)}, {"saved", u, 16}, {"dx", dx, 2},
+                                   {"da", da, size_of(param_dtype)}, {"db", db, size_of(param_dtype)}, {"adapter_ids", adapter_ids, 4}, {"experts", experts, 4},
+                                   {"scaling", scaling, 4}, {"the plan", plan, 256}, {"the workspace", workspace, 256}}))
+    return off;
   const kq::LoraCall c{types_of(dtype, param_dtype), kq::LoraGroups{adapter_ids, experts, slots, n_adapters, n_experts, rows, scaling, scale},
                        x, x_row_stride, x_shared, K, N, rank, a, b, plan};
   return done(op, kq::launch_lora_backward(c, dy, dy_row_stride, u, dx, K, da, db, workspace, st));
