@@ -372,7 +372,7 @@ KQ_API int kq_moe_router_grouped_backward(const void* logits, int dtype, long lo
  *  plan: the entries in the order of their groups, made by kq_lora_plan in kq_lora_plan_bytes(rows, n_adapters * n_experts)
  *    bytes of device memory (256-byte aligned) for the same adapter_ids, experts, rows, slots, n_adapters, n_experts. Needed by
  *    kq_lora_backward unless adapter_ids and experts are both NULL; kq_lora_update takes NULL too, but then looks for the rows of each
- *    group in every call: meant for up to 128 entries.
+ *    group in every call: meant for up to 128 entries, refused beyond 65536.
  *  workspace: kq_lora_backward_workspace_bytes(...) bytes, 256-byte aligned, private to the call until it completes.
  *  The same call gives the same bits. rows, K, N <= 2^30, n_adapters * n_experts <= 65535. */
 KQ_API size_t kq_lora_plan_bytes(long long rows, int n_groups);

@@ -29,6 +29,8 @@ int done(const char* what, cudaError_t e) {
 
 // rows, and values of a row: the kernels count them in 32 bits, some steps ahead of the last
 constexpr int kMost = 1 << 30;
+// rows without an order of their entries: every cluster looks through all indices, rows x rows reads in all
+constexpr int kMostDirect = 1 << 16;
 
 struct Operand {
   const char* name;
@@ -163,6 +165,8 @@ int kq_lora_update(const void* x, int dtype, long long rows, int K, long long x_
   const int rc = lora_check(op, dtype, param_dtype, rows, K, N, rank, slots, n_adapters, n_experts, adapter_ids, experts, plan, plan_bytes);
   if (rc != KQ_OK || rows == 0) return rc;
   if (!x || !a || !b || !y || !out) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] null pointer.", op);
+  if ((adapter_ids != nullptr || experts != nullptr) && plan == nullptr && rows > kMostDirect)
+    return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] needs the plan of its indices beyond %d rows.", op, kMostDirect);
   if (int off = aligned_check(op, {{"x", x, 2}, {"a", a, size_of(param_dtype)}, {"b", b, size_of(param_dtype)}, {"y", y, 2}, {"out", out, 2}, {"saved", u, 16},
                                    {"adapter_ids", adapter_ids, 4}, {"experts", experts, 4}, {"scaling", scaling, 4}, {"the plan", plan, 256}}))
     return off;

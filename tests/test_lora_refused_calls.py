@@ -1,4 +1,5 @@
-"""What the C entries of the low-rank adapters and the grouped router refuse before any launch: operands off their alignment."""
+"""What the C entries of the low-rank adapters and the grouped router refuse before any launch: operands off their alignment, long calls
+without an order of their entries."""
 import pytest
 
 from mlx_kquant_b200 import _lib
@@ -40,3 +41,8 @@ def test_router_off_alignment():
     back = lambda logits=P, idx=P, dw=P, dl=P: L.kq_moe_router_grouped_backward(logits, F16, 2, 16, 2, b"sigmoid", 1, 1.0, idx, dw, dl, None)  # noqa: E731
     for kw in (dict(logits=P + 1), dict(idx=P + 1), dict(dw=P + 2), dict(dl=P + 1)):
         assert back(**kw) == BAD and b"aligned" in L.kq_last_error(), kw
+
+
+def test_long_calls_need_the_order_of_their_entries():
+    for rows in (65537, 2 ** 24, 2 ** 29 + 1, 2 ** 30):
+        assert update(rows=rows) == BAD and b"plan" in L.kq_last_error()
