@@ -116,8 +116,10 @@ PyObject* qmm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// a plain, dense tensor on the current device
-bool ready(const at::Tensor& t) { return plain(t) && t.is_contiguous() && t.device().index() == c10::cuda::current_device(); }
+// a plain, dense tensor on the current device, without a forward-mode tangent (which the Python form refuses)
+bool ready(const at::Tensor& t) {
+  return plain(t) && t.is_contiguous() && t.device().index() == c10::cuda::current_device() && !t._fw_grad(0).defined();
+}
 
 bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
 

@@ -9,6 +9,7 @@ rounding to y's dtype.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import KQ_BF16, KQ_F16, KQ_F32, check
@@ -41,6 +42,12 @@ def _overlap(t: torch.Tensor, out: torch.Tensor) -> bool:
     t0, o0 = t.data_ptr(), out.data_ptr()
     t1 = t0 + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
     return t0 < o0 + out.numel() * out.element_size() and o0 < t1
+
+
+def _refuse_tangents(op, *tensors) -> None:
+    """Forward-mode differentiation, for which there is no rule: a tangent would be left out in silence."""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"[mlx_kquant.{op}] has no forward-mode derivative; differentiate it backwards.")
 
 
 def _i32(t: torch.Tensor, device) -> torch.Tensor:
@@ -164,6 +171,7 @@ class _Empty(torch.autograd.Function):
 def _update(op, y, x, a, b, call, scaling, out, stream):
     """The checks that both forms share, and the call."""
     dev = x.device
+    _refuse_tangents(op, y, x, a, b, scaling)
     if y.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"[mlx_kquant.{op}] y must be float16 or bfloat16 but is {y.dtype}.")
     if x.dtype != y.dtype:

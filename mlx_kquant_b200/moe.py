@@ -13,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .lora import _refuse_tangents
 from .ops import _on_device, _stream_ptr, gather_qmm
 
 
@@ -942,6 +943,7 @@ def moe_router_grouped(logits, top_k, n_groups=1, top_groups=1, *, scoring="sigm
     args = (top_k, n_groups, top_groups, scoring, bias, group_top, bool(norm_topk_prob), float(scale))
     if not logits.is_cuda:
         return _route_grouped_host(logits, *args)
+    _refuse_tangents(op, logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteGrouped.apply(logits, args)
     return _route_grouped(logits, *args)
