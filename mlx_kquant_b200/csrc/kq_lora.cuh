@@ -104,14 +104,17 @@ __device__ __forceinline__ uint32_t round_pair(float f0, float f1, __half) {
   const __half2 v = __floats2half2_rn(f0, f1);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// The leading bits of two floats as a bf16 pair, cut off (never rounded up to infinity), and what is left of them. FINITE: of
-// an infinity NaN is left, else nothing.
+// Two floats as the nearest bf16 pair, and what is left of them: 2^-8 of them at most, so that of two such splits' products the one of
+// both rests, which the products with two terms leave away, is below 2^-16. (Cut off, the rests were up to 2^-7 and never turned
+// down, the product left away up to 2^-14.) FINITE: of an infinity NaN is left, else nothing. (The last 2^-8 below the largest float
+// round to infinity.)
 template <bool FINITE>
 __device__ __forceinline__ uint32_t take_bf16(float& f0, float& f1) {
-  const uint32_t b0 = __float_as_uint(f0) & 0xffff0000u, b1 = __float_as_uint(f1) & 0xffff0000u;
-  f0 = !FINITE && fabsf(f0) == INFINITY ? 0.f : f0 - __uint_as_float(b0);
-  f1 = !FINITE && fabsf(f1) == INFINITY ? 0.f : f1 - __uint_as_float(b1);
-  return __byte_perm(b0, b1, 0x7632);
+  const uint32_t t = round_bf16(f0, f1);
+  const float t0 = __uint_as_float(t << 16), t1 = __uint_as_float(t & 0xffff0000u);
+  f0 = !FINITE && fabsf(t0) == INFINITY ? 0.f : f0 - t0;
+  f1 = !FINITE && fabsf(t1) == INFINITY ? 0.f : f1 - t1;
+  return t;
 }
 // N bf16 terms of the pair (f0, f1)
 template <int N, bool FINITE = false>
