@@ -362,7 +362,8 @@ KQ_API int kq_moe_router_grouped_backward(const void* logits, int dtype, long lo
  * expert is outside [0, n_experts) has none: its row of out is y's. f = scale * scaling[adapter] (scaling: float32, or NULL: 1).
  *  kq_lora_update: out[e] = y[e] + f (x[e] . a[g]^T) . b[g]^T; x rows of K values (x_shared != 0: one row per token, else one per
  *    entry), a [n_adapters, n_experts, rank, K], b [n_adapters, n_experts, N, rank], y and out rows of N values; out may be y.
- *    float32 sums, one rounding to out. saved: NULL, or kq_lora_saved_bytes(rows, rank, param_dtype) bytes, 16-byte aligned, that
+ *    float32 sums, one rounding to out; x . a^T enters the second product with 16 bits, and float32 parameters there likewise (the
+ *    same in kq_lora_backward for dy . b). What an infinity reaches is infinite or NaN. saved: NULL, or kq_lora_saved_bytes(rows, rank, param_dtype) bytes, 16-byte aligned, that
  *    receive x . a^T for the gradient (as bf16 terms: 24 bits of it beside float32 parameters, 16 beside others).
  *  kq_lora_backward, from dy [rows, N] and that: dx (rows of x, contiguous in K) = f (dy . b[g]) . a[g], summed over a token's slots
  *    where x_shared; da and db, of the parameters' type and shape, whole (zero for groups without entries). Each may be NULL. What

@@ -9,7 +9,7 @@
 //
 // float32 parameters are split into bf16 terms of 8 bits as they are read from shared memory: three where the result is kept in
 // float32 (u), two where it is rounded to 16 bits; fp16 rows are then two bf16 terms, exactly. u enters the second product as two
-// terms of the row's type, fp16 ones under a power of two per row. It is saved for the gradients as three bf16 terms beside float32
+// terms of the row's type, fp16 ones under a power of two per row: 16 bits. It is saved for the gradients as three bf16 terms beside float32
 // parameters, as two beside 16-bit ones, whose gradients are rounded to 16 bits.
 #pragma once
 

@@ -4,7 +4,8 @@ expert stack (`moe.gather_lora_update`), with their gradients.
 Adapter g of a projection [N, K] is a pair a[g] [r, K], b[g] [N, r]; a row x of a request that uses it gets
 ``y + s[g] * (x @ a[g].T) @ b[g].T`` on top of the projection's y. The rows of a batch may all use different adapters, and some
 none. All arithmetic happens in the CUDA library (kq_lora_update, kq_lora_backward in include/kquant_b200.h): float32 sums, one
-rounding to y's dtype.
+rounding to y's dtype, and between the two products x @ a.T (in the gradient dy @ b) with 16 bits, float32 parameters likewise in the
+second of them. What an infinity among the operands reaches is infinite or NaN.
 """
 from __future__ import annotations
 
@@ -231,9 +232,9 @@ def lora_update(y, x, a, b, adapter_ids=None, scaling=None, *, out=None, stream=
     for all rows below); outside [0, G): no adapter, the row stays y's. None: adapter 0 for every row. scaling: a number, or
     a tensor [G]; None: 1.
 
-    Returns a tensor like y, or writes to `out`, which may be y but overlaps nothing else. Differentiable in y, x, a and b (not with `out` or `stream`). The
-    same call gives the same bits. A training step can be captured into a CUDA graph; as for every operator of torch, no eager
-    autograd graph of the same leaves may be alive then."""
+    Returns a tensor like y, or writes to `out`, which may be y but overlaps nothing else. Differentiable backwards in y, x, a and b (not
+    with `out` or `stream`). The same call gives the same bits. A training step can be captured into a CUDA graph; as for every operator
+    of torch, no eager autograd graph of the same leaves may be alive then."""
     if out is None and stream is None:
         done = front_update(y, x, a, b, adapter_ids, scaling, None)
         if done is not None:
