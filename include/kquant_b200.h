@@ -393,6 +393,10 @@ KQ_API int kq_lora_backward(const void* dy, int dtype, long long rows, int N, lo
                             const float* scaling, float scale, const void* saved, void* dx, void* da, void* db, const void* plan,
                             size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
+/* kq_clear_rows: rows of y ([rows, N] of 2-byte values, dense) whose expert lies outside [0, n_experts) become zero, others are not
+ * touched: what kq_gather_qmm leaves unwritten. rows, N <= 2^30. */
+KQ_API int kq_clear_rows(void* y, long long rows, int N, const uint32_t* experts, int n_experts, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -214,4 +214,13 @@ int kq_lora_backward(const void* dy, int dtype, long long rows, int N, long long
   return done(op, kq::launch_lora_backward(c, dy, dy_row_stride, u, dx, K, da, db, workspace, st));
 }
 
+int kq_clear_rows(void* y, long long rows, int N, const uint32_t* experts, int n_experts, void* stream) {
+  const char* op = "clear_rows";
+  if (rows < 0 || rows > kMost || N < 1 || N > kMost || n_experts < 1) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] bad row, column or expert count.", op);
+  if (rows == 0) return KQ_OK;
+  if (!y || !experts) return fail(KQ_ERR_INVALID_ARGUMENT, "[mlx_kquant.%s] null pointer.", op);
+  if (int off = aligned_check(op, {{"y", y, 2}, {"experts", experts, 4}})) return off;
+  return done(op, kq::launch_clear_rows(y, (int)rows, N, experts, n_experts, static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

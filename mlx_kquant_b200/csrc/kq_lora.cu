@@ -488,6 +488,17 @@ __global__ void __launch_bounds__(kThreads) sum_slots_kernel(const float* part, 
   }
 }
 
+// Rows whose expert lies outside [0, E) become zero, the others are not touched. A warp a row.
+__global__ void __launch_bounds__(kThreads) clear_rows_kernel(uint16_t* y, int rows, int N, const uint32_t* experts, uint32_t E) {
+  wait_for_launch();
+  const int row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows || experts[row] < E) return;
+  uint16_t* p = y + (long long)row * N;
+  const int whole = (reinterpret_cast<uintptr_t>(p) & 15) == 0 ? N / 8 : 0;   // groups of 16 bytes
+  for (int c = lane; c < whole; c += 32) reinterpret_cast<uint4*>(p)[c] = make_uint4(0, 0, 0, 0);
+  for (int c = 8 * whole + lane; c < N; c += 32) p[c] = 0;
+}
+
 int sm_count() {
   static int known[16] = {};   // of the devices asked for so far
   int dev = 0, sms = 0;
@@ -625,6 +636,11 @@ cudaError_t launch_lora_sum_slots(const float* part, int slots, long long tokens
   const bool quads = cols % 4 == 0 && out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(part) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
   if (dtype == 1) return launch(sum_slots_kernel<__half>, grid, kThreads, 0, 0, st, part, slots, cols, static_cast<__half*>(out), out_stride, quads);
   return launch(sum_slots_kernel<bf16>, grid, kThreads, 0, 0, st, part, slots, cols, static_cast<bf16*>(out), out_stride, quads);
+}
+
+cudaError_t launch_clear_rows(void* y, int rows, int N, const uint32_t* experts, int n_experts, cudaStream_t st) {
+  return launch(clear_rows_kernel, dim3((unsigned)((rows + kThreads / 32 - 1) / (kThreads / 32))), kThreads, 0, 0, st, static_cast<uint16_t*>(y), rows, N, experts,
+                (uint32_t)n_experts);
 }
 
 cudaError_t launch_lora_forward(const LoraCall& c, const void* y, long long y_stride, void* out, long long out_stride, void* u,

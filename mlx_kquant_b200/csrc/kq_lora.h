@@ -96,6 +96,9 @@ cudaError_t launch_lora_wgrad(const LoraWgradArgs& a, int in_dtype, int out_f32,
 cudaError_t launch_lora_sum_slots(const float* part, int slots, long long tokens, int cols, void* out, long long out_stride, int dtype,
                                   cudaStream_t st);
 
+// rows of 16-bit values whose expert lies outside [0, n_experts) become zero
+cudaError_t launch_clear_rows(void* y, int rows, int N, const uint32_t* experts, int n_experts, cudaStream_t st);
+
 struct LoraCall {
   int types;                 // LoraTypes
   LoraGroups g;

@@ -11,8 +11,9 @@ import os
 
 import torch
 
+from . import _lib
 from . import ops as kq
-from .lora import _FrozenMatmul, lora_update
+from .lora import _FrozenMatmul, _i32, lora_update
 from .moe import gather_lora_update
 
 
@@ -203,21 +204,36 @@ class KQuantLoRALinear(torch.nn.Module):
         return f"rank={r}, n_adapters={n}"
 
 
+def _clear(y: torch.Tensor, indices: torch.Tensor, n_experts: int) -> torch.Tensor:
+    """y's rows of indices (int32) outside the stack, which the products leave unwritten, become zero."""
+    with kq._on_device(y.device):
+        kq.check(_lib.lib().kq_clear_rows(y.data_ptr(), indices.numel(), y.shape[-1], indices.data_ptr(), n_experts, kq._stream_ptr(None, y.device)))
+    return y
+
+
+def _routed(base: KQuantSwitchLinear, x: torch.Tensor, indices: torch.Tensor, sorted_indices: bool) -> torch.Tensor:
+    """The stack's products with rows of zeros where an index (int32) lies outside of it."""
+    E, near = base.weight.shape[0], indices
+    if base.bias is not None or sorted_indices:   # a bias is looked up for all, and the segments of sorted rows have no room for others
+        near = indices.clamp(0, E - 1)
+    return _clear(base(x, near, sorted_indices), indices, E)
+
+
 class _FrozenGather(torch.autograd.Function):
-    """gather_qmm over an expert stack with the gradient of its rows; the wire bytes have none. All indices lie in the stack."""
+    """_routed with the gradient of its rows; the wire bytes have none."""
 
     @staticmethod
-    def forward(ctx, x, w, scales, kquant_type, indices):
-        ctx.kquant_type, ctx.x_shape, ctx.dtype = kquant_type, x.shape, x.dtype
-        ctx.save_for_backward(w, indices)
-        return kq.gather_qmm(x.detach(), w, scales, kquant_type, rhs_indices=indices)
+    def forward(ctx, x, base, indices):
+        ctx.kquant_type, ctx.x_shape, ctx.dtype = base.kquant_type, x.shape, x.dtype
+        ctx.save_for_backward(base.weight, indices)
+        return _routed(base, x.detach(), indices, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         w, indices = ctx.saved_tensors
-        dx = kq.gather_qmm(dy, w, None, ctx.kquant_type, rhs_indices=indices, transpose=False)
-        return dx.float().sum_to_size(ctx.x_shape).to(ctx.dtype), None, None, None, None
+        dx = _clear(kq.gather_qmm(dy, w, None, ctx.kquant_type, rhs_indices=indices, transpose=False), indices, w.shape[0])
+        return dx.float().sum_to_size(ctx.x_shape).to(ctx.dtype), None, None
 
 
 class KQuantLoRASwitchLinear(torch.nn.Module):
@@ -246,14 +262,13 @@ class KQuantLoRASwitchLinear(torch.nn.Module):
                              and x.shape[1] in (1, indices.shape[1])):
             raise ValueError(f"KQuantLoRASwitchLinear: x must be [T, 1, 1, K] or [T, R, 1, K] with indices [T, R], or [B, 1, K] with "
                              f"indices [B], but x is {tuple(x.shape)} and indices {tuple(indices.shape)}.")
-        # the base's product leaves rows of other indices unwritten and looks for their bias: they take an expert's place and become zero
-        whole = indices.to(base.weight.device, indices.dtype if indices.dtype in (torch.int32, torch.int64) else torch.int64)
-        near = whole.clamp(0, base.weight.shape[0] - 1)   # (in order where the indices are)
+        if not x.is_cuda:
+            raise RuntimeError("KQuantLoRASwitchLinear: x must live on a CUDA device; there is no CPU path.")
+        indices = _i32(indices, base.weight.device)
         if torch.is_grad_enabled() and x.requires_grad:
-            y = base._add_bias(_FrozenGather.apply(x, base.weight, base.scales, base.kquant_type, near), near)
+            y = _FrozenGather.apply(x, base, indices)
         else:
-            y = base(x, near, sorted_indices)
-        y = torch.where((near == whole)[..., None, None], y, 0.0)
+            y = _routed(base, x, indices, sorted_indices)
         slots = indices.reshape(-1, 1) if flat else indices
         T, R = slots.shape
         rows = x.reshape(T, R, K) if flat or x.shape[1] == R else x.reshape(T, K)

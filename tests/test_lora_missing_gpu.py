@@ -105,3 +105,24 @@ def test_indices_out_of_range(dtype, grad):
     y = up(rows, many.to(dtype), of, sorted_indices=True)
     out = (many < 0) | (many >= 6)
     assert out.any() and not y[out].any() and y.isfinite().all() and y[~out].any(-1).all()
+
+
+@pytest.mark.parametrize("T,R,N", [(1, 1, 8), (5, 3, 7), (700, 8, 1001), (64, 1, 40000)])
+def test_clear_rows(T, R, N):
+    """All rows of indices outside the stack, to their ends, and no others; rows that start anywhere."""
+    from mlx_kquant_b200 import _lib
+    g = torch.Generator(device="cuda").manual_seed(T)
+    for skip in (0, 1, 8):
+        buf = torch.randn(T * R * N + 16, device="cuda", generator=g).half()
+        was = buf.clone()
+        idx = torch.randint(-1, 4, (T, R), device="cuda", generator=g, dtype=torch.int32)
+        _lib.check(_lib.lib().kq_clear_rows(buf.data_ptr() + 2 * skip, T * R, N, idx.data_ptr(), 3, torch.cuda.current_stream().cuda_stream))
+        want = was.clone()
+        want[skip:skip + T * R * N].view(T * R, N)[((idx < 0) | (idx > 2)).view(-1)] = 0
+        assert torch.equal(buf, want)
+
+
+def test_host_rows_are_refused():
+    up = layer()
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        up(torch.zeros(2, 1, 1, 256), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))

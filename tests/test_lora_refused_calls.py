@@ -43,6 +43,13 @@ def test_router_off_alignment():
         assert back(**kw) == BAD and b"aligned" in L.kq_last_error(), kw
 
 
+def test_clear_rows():
+    call = lambda y=P, rows=4, n=8, experts=P, E=2: L.kq_clear_rows(y, rows, n, experts, E, None)  # noqa: E731
+    for kw in (dict(y=None), dict(experts=None), dict(rows=-1), dict(rows=2 ** 30 + 1), dict(n=0), dict(E=0), dict(y=P + 1), dict(experts=P + 2)):
+        assert call(**kw) == BAD and b"[mlx_kquant.clear_rows]" in L.kq_last_error(), kw
+    assert call(rows=0) == 0
+
+
 def test_long_calls_need_the_order_of_their_entries():
     for rows in (65537, 2 ** 24, 2 ** 29 + 1, 2 ** 30):
         assert update(rows=rows) == BAD and b"plan" in L.kq_last_error()
